@@ -202,6 +202,64 @@ int s2_shared_linear(s2_context* ctx, int M0, int M1, int N, int K, const void* 
                      const float* bias, int epilogue, const float* gate, int out_dtype, void* out0, void* out1);
 
 /* ---------------------------------------------------------------------------
+ * Linear with its epilogue fused (no single counterpart in the reference,
+ * whose graphs run ncnn's InnerProduct / Gemm, activation and BinaryOp layers
+ * one after another):
+ *   out[r][n] = residual[r][n] + gate[n] * act(sum_k A[r][k] W[n][k] + bias[n])
+ * A bf16 [M][K] with row stride lda, W bf16 [N][K] with row stride ldw
+ * (elements; both strides multiples of 8, both bases 16-byte aligned; values
+ * between K and the stride are never used), fp32 accumulation.  Any M >= 0
+ * (0 does nothing), N >= 1 and K >= 1.  out [M][N] of out_dtype with row
+ * stride ldo, rounded once; any base aligned to its element (bases and row
+ * strides of 16 bytes' multiples are fastest).  residual: out_dtype, may be
+ * out itself with the same stride (in place); otherwise out overlaps no
+ * input.  Accumulation order depends on the sizes only: the same call gives
+ * the same bits.  Enqueues one kernel; no workspace; may be captured. */
+#define S2_ACT_NONE 0
+#define S2_ACT_SILU 1      /* x / (1 + e^-x) */
+#define S2_ACT_GELU_TANH 2 /* 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
+#define S2_ACT_GELU_ERF 3  /* 0.5 x (1 + erf(x / sqrt(2))) */
+typedef struct
+{
+    int act;              /* S2_ACT_* */
+    const float* bias;    /* fp32 [groups][N] or NULL (groups = 1 for s2_linear) */
+    const float* gate;    /* fp32 [groups][N] or NULL */
+    const void* residual; /* [rows][N] of out_dtype or NULL */
+    int64_t residual_ld;  /* its row stride */
+} s2_linear_epilogue;
+/* epilogue NULL: the bare product. */
+int s2_linear(s2_context* ctx, int M, int N, int K, const void* A, int64_t lda, const void* W, int64_t ldw,
+              const s2_linear_epilogue* epilogue, int out_dtype, void* out, int64_t ldo);
+/* The same product with one weight, bias and gate per group of rows (separate
+ * video and text weights, experts): rows offsets[g] <= r < offsets[g + 1] use
+ * W [groups][N][K] at row g * N of the stride ldw, bias[g] and gate[g].
+ * offsets: device int32 [groups + 1], non-decreasing within [0, rows], read
+ * when the kernel runs (no host copy); groups may be empty, rows before
+ * offsets[0] and from offsets[groups] on are left as they were.  An offset
+ * out of order or range leads no access outside the buffers: s2_status then
+ * returns -1 and out's rows are unspecified.  groups <= 1024. */
+int s2_grouped_linear(s2_context* ctx, int rows, int groups, const int* offsets, int N, int K, const void* A,
+                      int64_t lda, const void* W, int64_t ldw, const s2_linear_epilogue* epilogue, int out_dtype,
+                      void* out, int64_t ldo);
+
+/* Group norm with an activation over channels-last rows (the norm + SiLU in
+ * front of every convolution and of the attention of the VAE's blocks, whose
+ * graphs are outside the reference tree):
+ *   out[i][r][c] = act((x[i][r][c] - mean) / sqrt(var + eps) * gamma[c] + beta[c])
+ * with mean and biased variance of instance i (a frame) over its `rows` rows
+ * and the channels / groups consecutive channels of c's group, in fp32.  x:
+ * [instances * rows][channels] of in_dtype with row stride ldx (elements);
+ * out the same shape in out_dtype with row stride ldo, and may be x itself
+ * with the same type and stride; otherwise they do not overlap.  gamma, beta:
+ * fp32 [channels] or NULL.  channels is a multiple of groups; rows <= 2^30.
+ * 16-byte aligned bases and row strides are fastest.  NaN or Inf in a group
+ * makes that group's results NaN and no other's.  Enqueues one kernel; no
+ * workspace; may be captured. */
+int s2_group_norm(s2_context* ctx, int instances, int64_t rows, int channels, int groups, int in_dtype, const void* x,
+                  int64_t ldx, const float* gamma, const float* beta, float eps, int act, int out_dtype, void* out,
+                  int64_t ldo);
+
+/* ---------------------------------------------------------------------------
  * Block arithmetic around the layers (ops of the exported block graph).
  * ada_rmsnorm: out[r] (bf16) = x[r] * rsqrt(mean(x[r]^2) + eps) * scale + shift,
  * x fp32 [rows][D], shift/scale fp32 [D]. */

@@ -42,12 +42,18 @@ S2_EPI_STORE = 0
 S2_EPI_GELU_TANH = 1
 S2_EPI_GATE_RESIDUAL = 2
 
+S2_ACT_NONE = 0
+S2_ACT_SILU = 1
+S2_ACT_GELU_TANH = 2
+S2_ACT_GELU_ERF = 3
+
 # Every symbol include/seedvr2_cuda.h declares.
 EXPORTED = [
     "s2_init", "s2_destroy", "s2_set_stream", "s2_status", "s2_error_string", "s2_version", "s2_launch_count",
     "s2_profile_enable", "s2_profile_read",
     "s2_plan_build", "s2_plan_info", "s2_plan_copy", "s2_plan_free", "s2_plan_schedule_copy", "s2_debug_poke_schedule",
-    "s2_awa_forward", "s2_awa_forward_static", "s2_awa_static_status", "s2_shared_linear", "s2_ada_rmsnorm", "s2_ada_layernorm",
+    "s2_awa_forward", "s2_awa_forward_static", "s2_awa_static_status", "s2_shared_linear", "s2_linear", "s2_grouped_linear",
+    "s2_group_norm", "s2_ada_rmsnorm", "s2_ada_layernorm",
     "s2_convert_f32_bf16",
     "s2_count_nonfinite", "s2_binary_op", "s2_norm_f32", "s2_gelu_f32",
     "s2_dit_create", "s2_dit_free", "s2_dit_set_block_weights", "s2_dit_set_block_norm", "s2_dit_init_random",
@@ -111,6 +117,11 @@ class BlockHostWeights(C.Structure):
                                           "b_down", "qk_norm", "rope_freqs")]
 
 
+class LinearEpilogue(C.Structure):
+    _fields_ = [("act", C.c_int), ("bias", C.c_void_p), ("gate", C.c_void_p), ("residual", C.c_void_p),
+                ("residual_ld", C.c_int64)]
+
+
 class DenoiseOptions(C.Structure):
     _fields_ = [("steps", C.c_int), ("cfg_scale", C.c_float), ("cfg_rescale", C.c_float)]
 
@@ -160,6 +171,9 @@ def lib() -> C.CDLL:
                                         ip, vp, vp, vp]
     L.s2_awa_static_status.argtypes = [vp]
     L.s2_shared_linear.argtypes = [vp, ip, ip, ip, ip, vp, vp, vp, vp, ip, vp, ip, vp, vp]
+    L.s2_linear.argtypes = [vp, ip, ip, ip, vp, i64, vp, i64, C.POINTER(LinearEpilogue), ip, vp, i64]
+    L.s2_grouped_linear.argtypes = [vp, ip, ip, vp, ip, ip, vp, i64, vp, i64, C.POINTER(LinearEpilogue), ip, vp, i64]
+    L.s2_group_norm.argtypes = [vp, ip, i64, ip, ip, ip, vp, i64, vp, vp, C.c_float, ip, ip, vp, i64]
     L.s2_ada_rmsnorm.argtypes = [vp, ip, ip, vp, C.c_float, vp, vp, vp]
     L.s2_ada_layernorm.argtypes = [vp, ip, ip, vp, C.c_float, vp, vp, vp]
     L.s2_binary_op.argtypes = [vp, ip, ip, ip, vp, vp, ip, vp]
@@ -288,6 +302,12 @@ class Context:
             self.close()
         except Exception:
             pass
+
+    def set_stream(self, stream) -> None:
+        """Later calls enqueue on this torch stream (s2_set_stream)."""
+        if stream != self.stream:
+            check(lib().s2_set_stream(self.handle, C.c_void_p(stream.cuda_stream)), "s2_set_stream")
+            self.stream = stream
 
     def status(self) -> int:
         return lib().s2_status(self.handle)
@@ -425,6 +445,132 @@ def shared_linear(ctx: Context, a0, weight, bias=None, *, a1=None, epilogue=S2_E
                                epilogue, ptr(gate), out_dtype, out0.data_ptr(), ptr(out1))
     check(r, "s2_shared_linear")
     return out0, out1
+
+
+def _require(ok: bool, what: str) -> None:
+    if not ok:
+        raise S2Error(S2_ERR_INVALID, what)
+
+
+def _row_stride(t, what: str) -> int:
+    """Row stride (elements) of a tensor whose last dimension is dense and whose leading ones are one run of rows."""
+    shape, strides = t.shape, t.stride()
+    _require(len(shape) >= 2, what)
+    if t.numel() == 0:
+        return shape[-1]
+    _require(shape[-1] == 1 or strides[-1] == 1, what)
+    ld = None
+    run = 1  # rows below the dimension
+    for d in range(len(shape) - 2, -1, -1):
+        if shape[d] != 1:
+            if ld is None:
+                ld = strides[d]
+            _require(strides[d] == ld * run, what)
+        run *= shape[d]
+    return shape[-1] if ld is None else ld
+
+
+def _dtype_code(t, what: str) -> int:
+    import torch
+
+    _require(t.dtype in (torch.float32, torch.bfloat16), what)
+    return S2_DTYPE_F32 if t.dtype == torch.float32 else S2_DTYPE_BF16
+
+
+def _vector(t, shape, device, what: str):
+    """Address of an optional dense fp32 tensor of this shape."""
+    import torch
+
+    if t is None:
+        return None
+    _require(t.dtype == torch.float32 and tuple(t.shape) == tuple(shape) and t.is_contiguous() and t.device == device,
+             what)
+    return t.data_ptr()
+
+
+def _pitch16(k: int) -> int:
+    return (k + 7) // 8 * 8
+
+
+def _linear(ctx, what, a, weight, offsets, bias, act, gate, residual, out_dtype, out):
+    import torch
+
+    dev = torch.device("cuda", ctx.device)
+    grouped = offsets is not None
+    _require(a.dim() == 2 and weight.dim() == (3 if grouped else 2) and a.dtype == torch.bfloat16
+             and weight.dtype == torch.bfloat16 and a.device == dev and weight.device == dev
+             and weight.shape[-1] == a.shape[1], what)
+    rows, K = a.shape
+    N = weight.shape[-2]
+    groups = weight.shape[0] if grouped else 1
+    if grouped:
+        _require(offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.numel() == groups + 1
+                 and offsets.is_contiguous() and offsets.device == dev, what)
+    # a single row has no stride of its own
+    lda = a.stride(0) if rows > 1 else _pitch16(K)
+    _require(K == 1 or a.stride(1) == 1, what)
+    ldw = _row_stride(weight, what) if groups * N > 1 else _pitch16(K)
+    if out is None:
+        out = torch.empty((rows, N), device=dev,
+                          dtype=torch.float32 if out_dtype == S2_DTYPE_F32 else torch.bfloat16)
+    code = _dtype_code(out, what)
+    _require(out.dim() == 2 and tuple(out.shape) == (rows, N) and out.device == dev and (N == 1 or out.stride(1) == 1),
+             what)
+    vec = (groups, N) if grouped else (N,)
+    e = LinearEpilogue(int(act), _vector(bias, vec, dev, what), _vector(gate, vec, dev, what), None, 0)
+    if residual is not None:
+        _require(residual.dtype == out.dtype and residual.shape == out.shape and residual.device == dev
+                 and (N == 1 or residual.stride(1) == 1), what)
+        e.residual = residual.data_ptr()
+        e.residual_ld = residual.stride(0) if rows > 1 else N
+    ldo = out.stride(0) if rows > 1 else N
+    if grouped:
+        r = lib().s2_grouped_linear(ctx.handle, rows, groups, offsets.data_ptr(), N, K, a.data_ptr(), lda,
+                                    weight.data_ptr(), ldw, C.byref(e), code, out.data_ptr(), ldo)
+    else:
+        r = lib().s2_linear(ctx.handle, rows, N, K, a.data_ptr(), lda, weight.data_ptr(), ldw, C.byref(e), code,
+                            out.data_ptr(), ldo)
+    check(r, what)
+    return out
+
+
+def linear(ctx: Context, a, weight, bias=None, *, act=S2_ACT_NONE, gate=None, residual=None,
+           out_dtype=S2_DTYPE_BF16, out=None):
+    """residual + gate * act(a @ weight.T + bias): a [M, K] and weight [N, K] bf16 with dense rows of a stride that
+    is a multiple of 8, bias / gate fp32 [N], residual of the output's type (out itself to add in place)."""
+    return _linear(ctx, "s2_linear", a, weight, None, bias, act, gate, residual, out_dtype, out)
+
+
+def grouped_linear(ctx: Context, a, weight, offsets, bias=None, *, act=S2_ACT_NONE, gate=None, residual=None,
+                   out_dtype=S2_DTYPE_BF16, out=None):
+    """linear() with weight [G, N, K], bias / gate [G, N] of group g for rows offsets[g] <= r < offsets[g + 1]
+    (int32 CUDA tensor [G + 1]); other rows of out are left as they were (unset when out is made here)."""
+    _require(offsets is not None, "s2_grouped_linear")
+    return _linear(ctx, "s2_grouped_linear", a, weight, offsets, bias, act, gate, residual, out_dtype, out)
+
+
+def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=S2_ACT_NONE, out_dtype=None, out=None):
+    """act(group norm) of channels-last x [instances, ..., channels] (fp32 or bf16): statistics per instance and
+    channel group over the dimensions between; gamma / beta fp32 [channels].  out: x's shape (x itself in place)."""
+    import torch
+
+    what = "s2_group_norm"
+    dev = torch.device("cuda", ctx.device)
+    _require(x.dim() >= 2 and x.device == dev, what)
+    instances, channels = x.shape[0], x.shape[-1]
+    rows = 1
+    for n in x.shape[1:-1]:
+        rows *= n
+    code = _dtype_code(x, what)
+    if out is None:
+        out_dtype = code if out_dtype is None else out_dtype
+        out = torch.empty(x.shape, device=dev, dtype=torch.float32 if out_dtype == S2_DTYPE_F32 else torch.bfloat16)
+    _require(out.shape == x.shape and out.device == dev, what)
+    check(lib().s2_group_norm(ctx.handle, instances, rows, channels, int(groups), code, x.data_ptr(),
+                              _row_stride(x, what), _vector(gamma, (channels,), dev, what),
+                              _vector(beta, (channels,), dev, what), float(eps), int(act), _dtype_code(out, what),
+                              out.data_ptr(), _row_stride(out, what)), what)
+    return out
 
 
 def ada_rmsnorm(ctx: Context, x, eps, shift, scale, out=None):
