@@ -252,12 +252,17 @@ int s2_grouped_linear(s2_context* ctx, int rows, int groups, const int* offsets,
  * out the same shape in out_dtype with row stride ldo, and may be x itself
  * with the same type and stride; otherwise they do not overlap.  gamma, beta:
  * fp32 [channels] or NULL.  channels is a multiple of groups; rows <= 2^30.
- * 16-byte aligned bases and row strides are fastest.  NaN or Inf in a group
- * makes that group's results NaN and no other's.  Enqueues one kernel; no
- * workspace; may be captured. */
+ * channels <= 65536; 16-byte aligned bases and row strides are fastest.  NaN or
+ * Inf in a group makes that group's results NaN and no other's.  Activations of
+ * a bf16 result are within |z| 2^-12 of act(z) before its rounding.  The same
+ * call gives the same bits; it may be captured.
+ * workspace: s2_group_norm_workspace bytes (0 for small x, then NULL will do),
+ * 8-byte aligned, contents irrelevant before and after; calls that may run at
+ * the same time need one each. */
+size_t s2_group_norm_workspace(int instances, int64_t rows, int channels, int groups);
 int s2_group_norm(s2_context* ctx, int instances, int64_t rows, int channels, int groups, int in_dtype, const void* x,
                   int64_t ldx, const float* gamma, const float* beta, float eps, int act, int out_dtype, void* out,
-                  int64_t ldo);
+                  int64_t ldo, void* workspace, size_t workspace_bytes);
 
 /* ---------------------------------------------------------------------------
  * Block arithmetic around the layers (ops of the exported block graph).

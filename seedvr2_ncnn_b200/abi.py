@@ -53,7 +53,7 @@ EXPORTED = [
     "s2_profile_enable", "s2_profile_read",
     "s2_plan_build", "s2_plan_info", "s2_plan_copy", "s2_plan_free", "s2_plan_schedule_copy", "s2_debug_poke_schedule",
     "s2_awa_forward", "s2_awa_forward_static", "s2_awa_static_status", "s2_shared_linear", "s2_linear", "s2_grouped_linear",
-    "s2_group_norm", "s2_ada_rmsnorm", "s2_ada_layernorm",
+    "s2_group_norm", "s2_group_norm_workspace", "s2_ada_rmsnorm", "s2_ada_layernorm",
     "s2_convert_f32_bf16",
     "s2_count_nonfinite", "s2_binary_op", "s2_norm_f32", "s2_gelu_f32",
     "s2_dit_create", "s2_dit_free", "s2_dit_set_block_weights", "s2_dit_set_block_norm", "s2_dit_init_random",
@@ -173,7 +173,9 @@ def lib() -> C.CDLL:
     L.s2_shared_linear.argtypes = [vp, ip, ip, ip, ip, vp, vp, vp, vp, ip, vp, ip, vp, vp]
     L.s2_linear.argtypes = [vp, ip, ip, ip, vp, i64, vp, i64, C.POINTER(LinearEpilogue), ip, vp, i64]
     L.s2_grouped_linear.argtypes = [vp, ip, ip, vp, ip, ip, vp, i64, vp, i64, C.POINTER(LinearEpilogue), ip, vp, i64]
-    L.s2_group_norm.argtypes = [vp, ip, i64, ip, ip, ip, vp, i64, vp, vp, C.c_float, ip, ip, vp, i64]
+    L.s2_group_norm_workspace.argtypes = [ip, i64, ip, ip]
+    L.s2_group_norm_workspace.restype = C.c_size_t
+    L.s2_group_norm.argtypes = [vp, ip, i64, ip, ip, ip, vp, i64, vp, vp, C.c_float, ip, ip, vp, i64, vp, C.c_size_t]
     L.s2_ada_rmsnorm.argtypes = [vp, ip, ip, vp, C.c_float, vp, vp, vp]
     L.s2_ada_layernorm.argtypes = [vp, ip, ip, vp, C.c_float, vp, vp, vp]
     L.s2_binary_op.argtypes = [vp, ip, ip, ip, vp, vp, ip, vp]
@@ -566,10 +568,16 @@ def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=
         out_dtype = code if out_dtype is None else out_dtype
         out = torch.empty(x.shape, device=dev, dtype=torch.float32 if out_dtype == S2_DTYPE_F32 else torch.bfloat16)
     _require(out.shape == x.shape and out.device == dev, what)
+    need = lib().s2_group_norm_workspace(instances, rows, channels, int(groups))
+    ws = None
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        if ctx.stream != torch.cuda.current_stream(dev):
+            ws.record_stream(ctx.stream)
     check(lib().s2_group_norm(ctx.handle, instances, rows, channels, int(groups), code, x.data_ptr(),
                               _row_stride(x, what), _vector(gamma, (channels,), dev, what),
                               _vector(beta, (channels,), dev, what), float(eps), int(act), _dtype_code(out, what),
-                              out.data_ptr(), _row_stride(out, what)), what)
+                              out.data_ptr(), _row_stride(out, what), ptr(ws), need), what)
     return out
 
 

@@ -1,9 +1,18 @@
 // Activations of the linear and group norm epilogues (S2_ACT_*), on fp32
-// values.  The sigmoid forms are written as a quotient with one exponential:
-// x / (1 + e^-t) has no cancellation, so its error stays at a few units of
-// 2^-24 of the result where an fp32 output keeps it; tanh.approx (error
-// 2^-11) would show there.  x -> -inf gives 0 (the quotient's denominator
-// overflows to inf before x does) and NaN stays NaN.
+// values held as pairs (packed f32x2 arithmetic).
+//
+// Exact form: x sigmoid(t) = x / (1 + e^-t).  No cancellation, so the error
+// stays at a few units of 2^-24 of the result, where an fp32 output keeps it.
+// Four values share one reciprocal -- 1/a = b c d / (a b c d) -- so a value
+// costs 1.25 special-function operations instead of 2 (an SM starts 16 a
+// clock).  For that t is held at -21 and above, which keeps the product of
+// four finite: further out the result is below 1e-9 |x| either way.  A NaN t
+// becomes -21 there, so a NaN value reaches only itself.
+//
+// Fast form, for bf16 results: sigmoid(t) = (1 + tanh(t / 2)) / 2 with
+// tanh.approx, one special-function operation and no reciprocal.  Its error of
+// 2^-11 leaves |x| 2^-12, a sixteenth of the half step that rounding x itself
+// to bf16 would cost.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -12,46 +21,127 @@
 
 namespace s2 {
 
-// x * sigmoid(t)
-__device__ __forceinline__ float times_sigmoid(float x, float t)
+__device__ __forceinline__ float rcp_approx(float x)
 {
-    return __fdividef(x, 1.f + __expf(-t));
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-template <int ACT>
-__device__ __forceinline__ float activate_one(float x)
+__device__ __forceinline__ float ex2_approx(float x)
 {
-    if (ACT == S2_ACT_SILU) return times_sigmoid(x, x);
-    if (ACT == S2_ACT_GELU_TANH)
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float tanh_of(float x)
+{
+    float y;
+    asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float2 splat(float v)
+{
+    return make_float2(v, v);
+}
+
+constexpr float kSqrt2OverPi = 0.7978845608028654f;
+constexpr float kGeluCubic = 0.044715f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// v = act(v), exact form
+template <int ACT, int N>
+__device__ __forceinline__ void activate(float2 (&v)[N])
+{
+    if constexpr (ACT == S2_ACT_GELU_ERF)
     {
-        // 0.5 x (1 + tanh(u)) = x sigmoid(2u), u = sqrt(2/pi) (x + 0.044715 x^3)
-        const float k = 2.f * 0.7978845608028654f;
-        return times_sigmoid(x, k * x * (1.f + 0.044715f * x * x));
+#pragma unroll
+        for (int j = 0; j < N; j++)
+        {
+            v[j].x = 0.5f * v[j].x * (1.f + erff(v[j].x * 0.70710678118654752f));
+            v[j].y = 0.5f * v[j].y * (1.f + erff(v[j].y * 0.70710678118654752f));
+        }
     }
-    if (ACT == S2_ACT_GELU_ERF) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-    return x;
+    else if constexpr (ACT != S2_ACT_NONE)
+    {
+        constexpr int H = N % 2 == 0 ? 2 : 1; // pairs that share a reciprocal
+#pragma unroll
+        for (int j = 0; j < N; j += H)
+        {
+            float2 a[2] = {splat(1.f), splat(1.f)}; // 1 + e^-t
+#pragma unroll
+            for (int i = 0; i < H; i++)
+            {
+                const float2 x = v[j + i];
+                float2 t; // -t log2(e)
+                if constexpr (ACT == S2_ACT_SILU)
+                    t = __fmul2_rn(x, splat(-kLog2e));
+                else
+                {
+                    // 0.5 x (1 + tanh(u)) = x sigmoid(2u), u = sqrt(2/pi) (x + 0.044715 x^3)
+                    const float k = -2.f * kLog2e * kSqrt2OverPi;
+                    t = __fmul2_rn(x, __ffma2_rn(__fmul2_rn(x, splat(k * kGeluCubic)), x, splat(k)));
+                }
+                a[i] = __fadd2_rn(make_float2(ex2_approx(fminf(t.x, 30.3f)), ex2_approx(fminf(t.y, 30.3f))), splat(1.f));
+            }
+            const float ab = a[0].x * a[0].y, cd = a[1].x * a[1].y;
+            const float r = rcp_approx(ab * cd);
+            const float rab = r * cd, rcd = r * ab;
+            v[j].x *= rab * a[0].y;
+            v[j].y *= rab * a[0].x;
+            if constexpr (H == 2)
+            {
+                v[j + 1].x *= rcd * a[1].y;
+                v[j + 1].y *= rcd * a[1].x;
+            }
+        }
+    }
 }
 
-// The activation is uniform over a launch: one branch per N values.
+// Whether the fast form below takes this activation's argument halved.
+constexpr bool fast_halves(int act)
+{
+    return act == S2_ACT_SILU || act == S2_ACT_GELU_TANH;
+}
+
+// h = act(x), fast form, from h = x / 2 where fast_halves(ACT), else from x
+template <int ACT, int N>
+__device__ __forceinline__ void activate_fast(float2 (&h)[N])
+{
+    if constexpr (fast_halves(ACT))
+    {
+#pragma unroll
+        for (int j = 0; j < N; j++)
+        {
+            float2 t = h[j];
+            if constexpr (ACT == S2_ACT_GELU_TANH)
+                t = __fmul2_rn(t, __ffma2_rn(__fmul2_rn(t, splat(8.f * kSqrt2OverPi * kGeluCubic)), t, splat(2.f * kSqrt2OverPi)));
+            h[j] = __ffma2_rn(h[j], make_float2(tanh_of(t.x), tanh_of(t.y)), h[j]);
+        }
+    }
+    else
+        activate<ACT>(h);
+}
+
+// Exact form of N values, the activation given at run time.
 template <int N>
 __device__ __forceinline__ void activate(float (&v)[N], int act)
 {
-    switch (act)
-    {
-    case S2_ACT_SILU:
+    if (act == S2_ACT_NONE) return;
+    constexpr int P = (N + 1) / 2;
+    float2 p[P];
 #pragma unroll
-        for (int j = 0; j < N; j++) v[j] = activate_one<S2_ACT_SILU>(v[j]);
-        break;
-    case S2_ACT_GELU_TANH:
+    for (int j = 0; j < P; j++) p[j] = make_float2(v[2 * j], 2 * j + 1 < N ? v[(2 * j + 1) % N] : 0.f);
+    if (act == S2_ACT_SILU)
+        activate<S2_ACT_SILU>(p);
+    else if (act == S2_ACT_GELU_TANH)
+        activate<S2_ACT_GELU_TANH>(p);
+    else
+        activate<S2_ACT_GELU_ERF>(p);
 #pragma unroll
-        for (int j = 0; j < N; j++) v[j] = activate_one<S2_ACT_GELU_TANH>(v[j]);
-        break;
-    case S2_ACT_GELU_ERF:
-#pragma unroll
-        for (int j = 0; j < N; j++) v[j] = activate_one<S2_ACT_GELU_ERF>(v[j]);
-        break;
-    default: break;
-    }
+    for (int j = 0; j < N; j++) v[j] = j & 1 ? p[j / 2].y : p[j / 2].x;
 }
 
 } // namespace s2

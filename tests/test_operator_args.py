@@ -60,9 +60,9 @@ def test_linear_accepts(s2lib, ctx):
 
 
 def _norm(s2lib, ctx, *, instances=2, rows=5, channels=32, groups=4, in_dtype=1, x=BASE, ldx=32, gamma=None, beta=None,
-          eps=1e-6, act=0, out_dtype=1, out=OUT, ldo=32):
+          eps=1e-6, act=0, out_dtype=1, out=OUT, ldo=32, ws=1 << 28, ws_bytes=1 << 30):
     return s2lib.lib().s2_group_norm(ctx, instances, rows, channels, groups, in_dtype, x, ldx, gamma, beta, eps, act,
-                                     out_dtype, out, ldo)
+                                     out_dtype, out, ldo, ws, ws_bytes)
 
 
 BAD_NORM = [
@@ -70,7 +70,8 @@ BAD_NORM = [
     {"ldx": 31}, {"ldo": 31}, {"x": None}, {"out": None}, {"x": BASE + 1}, {"x": BASE + 2, "in_dtype": 0},
     {"out": OUT + 1}, {"out": OUT + 2, "out_dtype": 0}, {"in_dtype": 2}, {"out_dtype": -1}, {"act": 4}, {"act": -1},
     {"eps": -1.0}, {"eps": float("nan")}, {"gamma": BASE + 2}, {"beta": BASE + 1}, {"out": BASE, "out_dtype": 0},
-    {"out": BASE, "ldo": 40},
+    {"out": BASE, "ldo": 40}, {"channels": 65568, "ldx": 65568, "ldo": 65568}, {"ws": (1 << 28) + 4},
+    {"rows": 10**6, "ws": None}, {"rows": 10**6, "ws_bytes": 8},
 ]
 
 
@@ -85,6 +86,19 @@ def test_group_norm_accepts(s2lib, ctx):
         assert _norm(s2lib, ctx, **good) == s2lib.S2_ERR_CUDA, good
     for empty in ({"instances": 0}, {"rows": 0}):
         assert _norm(s2lib, ctx, **empty) == s2lib.S2_OK
+
+
+def test_group_norm_workspace(s2lib, ctx):
+    size = s2lib.lib().s2_group_norm_workspace
+    assert size(1, 256, 512, 32) == 0 and size(0, 5, 8, 1) == 0 and size(1, 5, 8, 3) == 0
+    assert _norm(s2lib, ctx, ws=None, ws_bytes=0) == s2lib.S2_ERR_CUDA, "small x needs none"
+    for shape in ((6, 14400, 512, 32), (1, 10**9, 8, 8), (1000, 3, 4096, 4096), (70000, 1, 32, 1)):
+        i, r, c, g = shape
+        need = size(*shape)
+        assert need % 8 == 0 and 8 * i * g <= need <= 8 * g * max(i, 444)
+        args = dict(instances=i, rows=r, channels=c, groups=g, ldx=c, ldo=c)
+        assert _norm(s2lib, ctx, ws_bytes=need, **args) == s2lib.S2_ERR_CUDA
+        assert _norm(s2lib, ctx, ws_bytes=need - 1, **args) == s2lib.S2_ERR_INVALID
 
 
 def test_row_strides(s2lib):
