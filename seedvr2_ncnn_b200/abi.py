@@ -456,10 +456,11 @@ def _require(ok: bool, what: str) -> None:
 
 def _row_stride(t, what: str) -> int:
     """Row stride (elements) of a tensor whose last dimension is dense and whose leading ones are one run of rows."""
-    shape, strides = t.shape, t.stride()
+    shape = t.shape
     _require(len(shape) >= 2, what)
-    if t.numel() == 0:
+    if t.is_contiguous() or t.numel() == 0:
         return shape[-1]
+    strides = t.stride()
     _require(shape[-1] == 1 or strides[-1] == 1, what)
     ld = None
     run = 1  # rows below the dimension
@@ -472,66 +473,70 @@ def _row_stride(t, what: str) -> int:
     return shape[-1] if ld is None else ld
 
 
+_codes = {}
+
+
 def _dtype_code(t, what: str) -> int:
-    import torch
+    if not _codes:
+        import torch
 
-    _require(t.dtype in (torch.float32, torch.bfloat16), what)
-    return S2_DTYPE_F32 if t.dtype == torch.float32 else S2_DTYPE_BF16
+        _codes.update({torch.float32: S2_DTYPE_F32, torch.bfloat16: S2_DTYPE_BF16})
+    code = _codes.get(t.dtype)
+    _require(code is not None, what)
+    return code
 
 
-def _vector(t, shape, device, what: str):
+def _vector(t, shape, device: int, what: str):
     """Address of an optional dense fp32 tensor of this shape."""
-    import torch
-
     if t is None:
         return None
-    _require(t.dtype == torch.float32 and tuple(t.shape) == tuple(shape) and t.is_contiguous() and t.device == device,
-             what)
+    _require(_dtype_code(t, what) == S2_DTYPE_F32 and t.shape == shape and t.get_device() == device
+             and t.is_contiguous(), what)
     return t.data_ptr()
 
 
-def _pitch16(k: int) -> int:
-    return (k + 7) // 8 * 8
+def _new(ctx, shape, code):
+    import torch
+
+    return torch.empty(shape, device=torch.device("cuda", ctx.device),
+                       dtype=torch.float32 if code == S2_DTYPE_F32 else torch.bfloat16)
+
+
+def _operand(t, dim: int, device: int, what: str) -> int:
+    """Row stride of a bf16 operand; a single row, which has none of its own, gets its length rounded up to 8."""
+    _require(t.dim() == dim and _dtype_code(t, what) == S2_DTYPE_BF16 and t.get_device() == device, what)
+    ld = _row_stride(t, what)
+    k = t.shape[-1]
+    return (k + 7) // 8 * 8 if t.numel() == k else ld
 
 
 def _linear(ctx, what, a, weight, offsets, bias, act, gate, residual, out_dtype, out):
-    import torch
-
-    dev = torch.device("cuda", ctx.device)
+    dev = ctx.device
     grouped = offsets is not None
-    _require(a.dim() == 2 and weight.dim() == (3 if grouped else 2) and a.dtype == torch.bfloat16
-             and weight.dtype == torch.bfloat16 and a.device == dev and weight.device == dev
-             and weight.shape[-1] == a.shape[1], what)
+    lda, ldw = _operand(a, 2, dev, what), _operand(weight, 3 if grouped else 2, dev, what)
     rows, K = a.shape
     N = weight.shape[-2]
+    _require(weight.shape[-1] == K, what)
     groups = weight.shape[0] if grouped else 1
-    if grouped:
-        _require(offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.numel() == groups + 1
-                 and offsets.is_contiguous() and offsets.device == dev, what)
-    # a single row has no stride of its own
-    lda = a.stride(0) if rows > 1 else _pitch16(K)
-    _require(K == 1 or a.stride(1) == 1, what)
-    ldw = _row_stride(weight, what) if groups * N > 1 else _pitch16(K)
     if out is None:
-        out = torch.empty((rows, N), device=dev,
-                          dtype=torch.float32 if out_dtype == S2_DTYPE_F32 else torch.bfloat16)
+        out = _new(ctx, (rows, N), out_dtype)
     code = _dtype_code(out, what)
-    _require(out.dim() == 2 and tuple(out.shape) == (rows, N) and out.device == dev and (N == 1 or out.stride(1) == 1),
-             what)
+    _require(out.shape == (rows, N) and out.get_device() == dev, what)
     vec = (groups, N) if grouped else (N,)
-    e = LinearEpilogue(int(act), _vector(bias, vec, dev, what), _vector(gate, vec, dev, what), None, 0)
+    e = LinearEpilogue(act, _vector(bias, vec, dev, what), _vector(gate, vec, dev, what), None, 0)
     if residual is not None:
-        _require(residual.dtype == out.dtype and residual.shape == out.shape and residual.device == dev
-                 and (N == 1 or residual.stride(1) == 1), what)
+        _require(residual.dtype == out.dtype and residual.shape == out.shape and residual.get_device() == dev, what)
         e.residual = residual.data_ptr()
-        e.residual_ld = residual.stride(0) if rows > 1 else N
-    ldo = out.stride(0) if rows > 1 else N
+        e.residual_ld = _row_stride(residual, what)
+    L = lib()
     if grouped:
-        r = lib().s2_grouped_linear(ctx.handle, rows, groups, offsets.data_ptr(), N, K, a.data_ptr(), lda,
-                                    weight.data_ptr(), ldw, C.byref(e), code, out.data_ptr(), ldo)
+        _require(str(offsets.dtype) == "torch.int32" and offsets.shape == (groups + 1,) and offsets.is_contiguous()
+                 and offsets.get_device() == dev, what)
+        r = L.s2_grouped_linear(ctx.handle, rows, groups, offsets.data_ptr(), N, K, a.data_ptr(), lda,
+                                weight.data_ptr(), ldw, C.byref(e), code, out.data_ptr(), _row_stride(out, what))
     else:
-        r = lib().s2_linear(ctx.handle, rows, N, K, a.data_ptr(), lda, weight.data_ptr(), ldw, C.byref(e), code,
-                            out.data_ptr(), ldo)
+        r = L.s2_linear(ctx.handle, rows, N, K, a.data_ptr(), lda, weight.data_ptr(), ldw, C.byref(e), code,
+                        out.data_ptr(), _row_stride(out, what))
     check(r, what)
     return out
 
@@ -554,30 +559,32 @@ def grouped_linear(ctx: Context, a, weight, offsets, bias=None, *, act=S2_ACT_NO
 def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=S2_ACT_NONE, out_dtype=None, out=None):
     """act(group norm) of channels-last x [instances, ..., channels] (fp32 or bf16): statistics per instance and
     channel group over the dimensions between; gamma / beta fp32 [channels].  out: x's shape (x itself in place)."""
-    import torch
-
     what = "s2_group_norm"
-    dev = torch.device("cuda", ctx.device)
-    _require(x.dim() >= 2 and x.device == dev, what)
-    instances, channels = x.shape[0], x.shape[-1]
+    dev = ctx.device
+    shape = x.shape
+    _require(len(shape) >= 2 and x.get_device() == dev, what)
+    instances, channels = shape[0], shape[-1]
     rows = 1
-    for n in x.shape[1:-1]:
+    for n in shape[1:-1]:
         rows *= n
     code = _dtype_code(x, what)
     if out is None:
-        out_dtype = code if out_dtype is None else out_dtype
-        out = torch.empty(x.shape, device=dev, dtype=torch.float32 if out_dtype == S2_DTYPE_F32 else torch.bfloat16)
-    _require(out.shape == x.shape and out.device == dev, what)
-    need = lib().s2_group_norm_workspace(instances, rows, channels, int(groups))
+        out = _new(ctx, shape, code if out_dtype is None else out_dtype)
+    out_code = _dtype_code(out, what)
+    _require(out.shape == shape and out.get_device() == dev, what)
+    L = lib()
+    need = L.s2_group_norm_workspace(instances, rows, channels, groups)
     ws = None
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        import torch
+
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
         if ctx.stream != torch.cuda.current_stream(dev):
             ws.record_stream(ctx.stream)
-    check(lib().s2_group_norm(ctx.handle, instances, rows, channels, int(groups), code, x.data_ptr(),
-                              _row_stride(x, what), _vector(gamma, (channels,), dev, what),
-                              _vector(beta, (channels,), dev, what), float(eps), int(act), _dtype_code(out, what),
-                              out.data_ptr(), _row_stride(out, what), ptr(ws), need), what)
+    vec = (channels,)
+    check(L.s2_group_norm(ctx.handle, instances, rows, channels, groups, code, x.data_ptr(), _row_stride(x, what),
+                          _vector(gamma, vec, dev, what), _vector(beta, vec, dev, what), eps, act, out_code,
+                          out.data_ptr(), _row_stride(out, what), ptr(ws), need), what)
     return out
 
 

@@ -51,6 +51,27 @@ constexpr float kSqrt2OverPi = 0.7978845608028654f;
 constexpr float kGeluCubic = 0.044715f;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// 0.5 x (1 + erf(x / sqrt 2)) without a branch (erff's two branches cost a warp
+// both, one element after another): with z = |x| / sqrt 2 and q = erfc(z) / 2,
+// the result is max(x, 0) - |x| q.  erfc by Abramowitz and Stegun 7.1.26,
+// absolute error 1.5e-7.  |x| above 30, where q is zero, is held there (no
+// inf times zero); the first term keeps NaN and +inf.
+__device__ __forceinline__ float2 gelu_erf(float2 x)
+{
+    const float2 ax = make_float2(fabsf(x.x), fabsf(x.y));
+    const float2 a = make_float2(fminf(ax.x, 30.f), fminf(ax.y, 30.f));
+    const float2 d = __ffma2_rn(a, splat(0.3275911f * 0.70710678f), splat(1.f));
+    const float2 t = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    float2 p = __ffma2_rn(t, splat(0.5f * 1.061405429f), splat(0.5f * -1.453152027f));
+    p = __ffma2_rn(t, p, splat(0.5f * 1.421413741f));
+    p = __ffma2_rn(t, p, splat(0.5f * -0.284496736f));
+    p = __ffma2_rn(t, p, splat(0.5f * 0.254829592f));
+    p = __fmul2_rn(t, p);
+    const float2 z2 = __fmul2_rn(__fmul2_rn(a, splat(-0.5f * kLog2e)), a);
+    p = __fmul2_rn(__fmul2_rn(p, a), make_float2(ex2_approx(z2.x), ex2_approx(z2.y)));
+    return make_float2(fmaf(0.5f, x.x + ax.x, -p.x), fmaf(0.5f, x.y + ax.y, -p.y));
+}
+
 // v = act(v), exact form
 template <int ACT, int N>
 __device__ __forceinline__ void activate(float2 (&v)[N])
@@ -58,11 +79,7 @@ __device__ __forceinline__ void activate(float2 (&v)[N])
     if constexpr (ACT == S2_ACT_GELU_ERF)
     {
 #pragma unroll
-        for (int j = 0; j < N; j++)
-        {
-            v[j].x = 0.5f * v[j].x * (1.f + erff(v[j].x * 0.70710678118654752f));
-            v[j].y = 0.5f * v[j].y * (1.f + erff(v[j].y * 0.70710678118654752f));
-        }
+        for (int j = 0; j < N; j++) v[j] = gelu_erf(v[j]);
     }
     else if constexpr (ACT != S2_ACT_NONE)
     {

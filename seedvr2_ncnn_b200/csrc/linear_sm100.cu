@@ -22,6 +22,15 @@ constexpr int A_BYTES = BM * BK * 2;
 constexpr int kMaxGroups = 1024;
 constexpr size_t kSmemLimit = 232448;
 
+// The tensor core adds into its fp32 accumulator without rounding to nearest:
+// over K = 10,240 an fp32 result is then off by 1.2e-5 of itself (5.2e-6
+// measured under a gate and a residual).  Where the result is fp32 and K is
+// longer than kLongK blocks, sums of kChunk blocks are therefore added up in
+// fp32 registers (or shared memory) instead, each while the tensor core works
+// on the next one.  A bf16 result rounds at 2^-9 and keeps one sum.
+constexpr int kChunk = 24;
+constexpr int kLongK = 24;
+
 struct LinearArgs
 {
     int rows, N, K, groups, num_kb, nblk;
@@ -38,49 +47,32 @@ struct LinearArgs
     int tma_res; // residual through its tensor map
     int stages;
     int group_m; // M blocks per raster group
-    int cluster; // linear_rows_kernel: K parts
+    int chunk_kb; // K blocks summed by the tensor core before the sum is taken over (see kChunk)
+    int cluster;  // linear_rows_kernel: K parts
+    int vec_out, vec_res; // linear_rows_kernel: four outputs / residuals at once
     int* status;
 };
 
-__device__ __forceinline__ void add_bias32(const LinearArgs& a, const float* bias, int n, float (&x)[32])
+// v[j] = vec[n + j], 0 past N
+template <int W>
+__device__ __forceinline__ void load_columns(const float* vec, int n, int N, float (&v)[W])
 {
-    if (n + 32 <= a.N && (reinterpret_cast<uintptr_t>(bias + n) & 15) == 0)
+    if (n + W <= N && (reinterpret_cast<uintptr_t>(vec + n) & 15) == 0)
     {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
+        for (int j = 0; j < W; j += 4)
         {
-            const float4 b = __ldg(reinterpret_cast<const float4*>(bias + n + j));
-            x[j] += b.x;
-            x[j + 1] += b.y;
-            x[j + 2] += b.z;
-            x[j + 3] += b.w;
+            const float4 b = __ldg(reinterpret_cast<const float4*>(vec + n + j));
+            v[j] = b.x;
+            v[j + 1] = b.y;
+            v[j + 2] = b.z;
+            v[j + 3] = b.w;
         }
     }
     else
     {
 #pragma unroll
-        for (int j = 0; j < 32; j++) x[j] += n + j < a.N ? __ldg(bias + n + j) : 0.f;
-    }
-}
-
-__device__ __forceinline__ void mul_gate32(const LinearArgs& a, const float* gate, int n, float (&x)[32])
-{
-    if (n + 32 <= a.N && (reinterpret_cast<uintptr_t>(gate + n) & 15) == 0)
-    {
-#pragma unroll
-        for (int j = 0; j < 32; j += 4)
-        {
-            const float4 g = __ldg(reinterpret_cast<const float4*>(gate + n + j));
-            x[j] *= g.x;
-            x[j + 1] *= g.y;
-            x[j + 2] *= g.z;
-            x[j + 3] *= g.w;
-        }
-    }
-    else
-    {
-#pragma unroll
-        for (int j = 0; j < 32; j++) x[j] *= n + j < a.N ? __ldg(gate + n + j) : 0.f;
+        for (int j = 0; j < W; j++) v[j] = n + j < N ? __ldg(vec + n + j) : 0.f;
     }
 }
 
@@ -182,8 +174,32 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity)
 }
 
 // ---------------------------------------------------------------- many rows
-constexpr int kEpiWarps = 8; // two per TMEM lane quarter, half the columns each
-constexpr int kTileThreads = 64 + 32 * kEpiWarps;
+// Warps: TMA, MMA, then eight for the epilogue, two per TMEM lane quarter with
+// half the columns each.  Where these hold sums of the accumulator in registers
+// (SUM) they begin at warp 4, so that setmaxnreg can give them what the first
+// four do not need: 104 + 2 x 200 = 3 x 168 registers per thread and warpgroup,
+// the 168 a thread that 384 threads are launched with.
+constexpr int kEpiWarps = 8;
+constexpr int kSumRegs = 200, kOtherRegs = 104, kLaunchRegs = 168;
+static_assert(kOtherRegs + 2 * kSumRegs == 3 * kLaunchRegs, "register split");
+constexpr int first_epilogue_warp(bool sum)
+{
+    return sum ? 4 : 2;
+}
+constexpr int tile_threads(bool sum)
+{
+    return 32 * (first_epilogue_warp(sum) + kEpiWarps);
+}
+template <int N>
+__device__ __forceinline__ void regs_increase()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_decrease()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 constexpr int kBox = 4096; // 32 rows x 128 bytes
 
 // CTAS = 2: a pair of CTAs (cluster of 2) computes 256 rows x BN columns with
@@ -205,6 +221,16 @@ struct TileShape
     }
 };
 
+// 32 lanes x 16 consecutive 32-bit columns -> 16 registers per thread.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
 // Byte of (row r, byte b) in a 128-byte-swizzled box.
 __device__ __forceinline__ int box_at(int r, int b)
 {
@@ -217,26 +243,124 @@ template <typename T>
 __device__ __forceinline__ void box_to_global(const uint8_t* box, T* out, int64_t ld, int rows, int cols, int lane)
 {
     constexpr int W = 128 / sizeof(T);
+#pragma unroll 8
     for (int r = 0; r < rows; r++)
 #pragma unroll
         for (int c = lane; c < W; c += 32)
             if (c < cols) out[r * ld + c] = *reinterpret_cast<const T*>(box + box_at(r, c * (int)sizeof(T)));
 }
-template <typename T>
-__device__ __forceinline__ void global_to_box(uint8_t* box, const T* in, int64_t ld, int rows, int cols, int lane)
+
+// A residual box in registers, one word a row (fp32: column `lane`; bf16:
+// columns `lane` and `lane + 32`), so that all of it is in flight at once.
+struct HeldBox
 {
-    constexpr int W = 128 / sizeof(T);
-    for (int r = 0; r < rows; r++)
+    uint32_t w[32];
+    __device__ void load(const LinearArgs& a, int row0, int n, int rows, int lane)
+    {
+        const int64_t ld = a.residual_ld;
+        if (a.out_f32)
+        {
+            const uint32_t* p = static_cast<const uint32_t*>(a.residual) + (int64_t)row0 * ld + n + lane;
 #pragma unroll
-        for (int c = lane; c < W; c += 32)
-            if (c < cols) *reinterpret_cast<T*>(box + box_at(r, c * (int)sizeof(T))) = in[r * ld + c];
+            for (int r = 0; r < 32; r++) w[r] = r < rows && n + lane < a.N ? p[r * ld] : 0u;
+        }
+        else
+        {
+            const uint16_t* p = static_cast<const uint16_t*>(a.residual) + (int64_t)row0 * ld + n + lane;
+#pragma unroll
+            for (int r = 0; r < 32; r++)
+            {
+                const uint32_t lo = r < rows && n + lane < a.N ? p[r * ld] : 0u;
+                const uint32_t hi = r < rows && n + lane + 32 < a.N ? p[r * ld + 32] : 0u;
+                w[r] = lo | hi << 16;
+            }
+        }
+    }
+    __device__ void put(const LinearArgs& a, uint8_t* box, int lane) const
+    {
+#pragma unroll
+        for (int r = 0; r < 32; r++)
+            if (a.out_f32)
+                *reinterpret_cast<uint32_t*>(box + box_at(r, lane * 4)) = w[r];
+            else
+            {
+                *reinterpret_cast<uint16_t*>(box + box_at(r, lane * 2)) = (uint16_t)w[r];
+                *reinterpret_cast<uint16_t*>(box + box_at(r, lane * 2 + 64)) = (uint16_t)(w[r] >> 16);
+            }
+    }
+};
+
+// W accumulator columns of this lane's row -> the result, in the box (srow: the
+// lane's row of it; col: the first column's place in the box).
+template <int W>
+__device__ __forceinline__ void finish(const LinearArgs& a, const float* x0, const float* bias, const float* gate, int n,
+                                       uint8_t* srow, int sw, int col)
+{
+    float x[W], v[W];
+#pragma unroll
+    for (int j = 0; j < W; j++) x[j] = x0[j];
+    if (bias)
+    {
+        load_columns<W>(bias, n, a.N, v);
+#pragma unroll
+        for (int j = 0; j < W; j++) x[j] += v[j];
+    }
+    activate<W>(x, a.act);
+    if (gate)
+    {
+        load_columns<W>(gate, n, a.N, v);
+#pragma unroll
+        for (int j = 0; j < W; j++) x[j] *= v[j];
+    }
+    if (a.out_f32)
+    {
+#pragma unroll
+        for (int j = 0; j < W; j += 4)
+        {
+            float4* p = reinterpret_cast<float4*>(srow + ((((col + j) >> 2) ^ sw) << 4));
+            float4 o = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+            if (a.residual)
+            {
+                const float4 r = *p;
+                o.x += r.x;
+                o.y += r.y;
+                o.z += r.z;
+                o.w += r.w;
+            }
+            *p = o;
+        }
+    }
+    else
+    {
+#pragma unroll
+        for (int j = 0; j < W; j += 8)
+        {
+            uint4* p = reinterpret_cast<uint4*>(srow + ((((col + j) >> 3) ^ sw) << 4));
+            if (a.residual)
+            {
+                const uint4 r = *p;
+                const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                {
+                    const float2 f = unpack_bf16x2(rw[e]);
+                    x[j + 2 * e] += f.x;
+                    x[j + 2 * e + 1] += f.y;
+                }
+            }
+            *p = make_uint4(pack_bf16x2(x[j], x[j + 1]), pack_bf16x2(x[j + 2], x[j + 3]),
+                            pack_bf16x2(x[j + 4], x[j + 5]), pack_bf16x2(x[j + 6], x[j + 7]));
+        }
+    }
 }
 
 // Epilogue of one warp over all of the CTA's units.  Boxes (32 rows x 128
 // bytes of output) run in a fixed sequence; each is combined in one of the
 // warp's R shared-memory boxes and written by one TMA store.  A residual box is
-// TMA-loaded R - 1 boxes ahead into the slot its result will leave from.
-template <int CTAS, int BN, int R>
+// TMA-loaded R - 1 boxes ahead into the slot its result will leave from, or
+// held in registers one box ahead where TMA cannot take it.  SUM (fp32 results,
+// long K): the accumulator's chunks are added up in registers first.
+template <int CTAS, int BN, int R, bool SUM>
 __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtensorMap* tmap_out,
                                               const CUtensorMap* tmap_res, UnitWalk<CTAS * BM, BN> walk,
                                               UnitWalk<CTAS * BM, BN> ahead, int first_unit, int step, int units,
@@ -244,11 +368,12 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
                                               uint64_t* tempty, uint32_t tmem_base, int quarter, int half, int lane,
                                               volatile int* abort_flag)
 {
-    const int esz = a.out_f32 ? 4 : 2;
-    const int box_cols = 128 / esz;
+    constexpr int COLS = BN / 2; // of a unit, per warp
+    const int box_cols = SUM ? 32 : (a.out_f32 ? 32 : 64);
     const int row_in = rank * BM + quarter * 32; // of the unit, this warp's first
-    const int c_lo = half * (BN / 2), c_hi = c_lo + BN / 2;
+    const int c_lo = half * COLS, c_hi = c_lo + COLS;
     const int sw = lane & 7;
+    const bool held = a.residual && !a.tma_res;
     // loader cursor (lane 0)
     int lu = first_unit, lc = c_lo, lq = 0;
     Unit lun{};
@@ -273,115 +398,96 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
         lq++;
         lc += box_cols;
     };
+    // a unit's residual boxes go to L2 a unit ahead
+    UnitWalk<CTAS * BM, BN> far = ahead;
+    auto prefetch_unit = [&](int u) {
+        if (u >= units) return;
+        const Unit p = far.decode(a, u);
+        if (p.m0 + row_in >= p.end) return;
+        for (int c = c_lo; c < c_hi && p.n0 + c < a.N; c += box_cols)
+            tma_prefetch_l2_2d(tmap_res, p.n0 + c, p.m0 + row_in);
+    };
     if (a.tma_res && lane == 0)
+    {
+        prefetch_unit(first_unit);
         for (int i = 0; i < R - 1; i++) issue_load();
+    }
 
     int q = 0, acc = 0;
     uint32_t acc_phase = 0;
-    bool ok = true;
-    for (int u = first_unit; u < units && ok; u += step)
-    {
+    auto wait_acc = [&]() {
         int w = 0;
         if (lane == 0) w = mbar_wait<true>(&tfull[acc], acc_phase, abort_flag, a.status) ? 1 : 0;
         w = __shfl_sync(0xffffffffu, w, 0);
-        if (!w) break;
         __syncwarp();
         tc_fence_after();
+        return w != 0;
+    };
+    auto release_acc = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0)
+        {
+            if (CTAS == 2)
+                mbar_arrive_cluster(mapa_shared(&tempty[acc], 0));
+            else
+                mbar_arrive(&tempty[acc]);
+        }
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+    };
+    bool ok = true;
+    for (int u = first_unit; u < units && ok; u += step)
+    {
         const Unit un = walk.decode(a, u);
         const int row0 = un.m0 + row_in;
         const int live_rows = min(32, un.end - row0);
         const float* bias = a.bias ? a.bias + (int64_t)un.group * a.N : nullptr;
         const float* gate = a.gate ? a.gate + (int64_t)un.group * a.N : nullptr;
-        const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
-#pragma unroll 1
-        for (int c = c_lo; c < c_hi && un.n0 + c < a.N && live_rows > 0; c += box_cols, q++)
-        {
+        const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        if (a.tma_res && lane == 0) prefetch_unit(u + step);
+        HeldBox next;
+        if (!SUM && held && live_rows > 0 && un.n0 + c_lo < a.N) next.load(a, row0, un.n0 + c_lo, live_rows, lane);
+
+        // box q of the warp, columns [c, c + box_cols) of the unit: from its
+        // slot's release to its store
+        auto open_box = [&](int c) {
             const int slot = q % R;
             uint8_t* box = stg + slot * kBox;
-            const int n = un.n0 + c;
-            const int live_cols = min(box_cols, a.N - n);
             if (a.tma_res)
             {
                 int r = 0;
                 if (lane == 0) r = mbar_wait<true>(&rfull[slot], (uint32_t)(q / R) & 1u, abort_flag, a.status) ? 1 : 0;
                 r = __shfl_sync(0xffffffffu, r, 0);
-                if (!r)
-                {
-                    ok = false;
-                    break;
-                }
+                return r != 0;
             }
-            else
+            if (lane == 0) bulk_wait_read<R - 1>(); // this slot's previous store has read it
+            __syncwarp();
+            if (held)
             {
-                if (lane == 0) bulk_wait_read<R - 1>(); // this slot's previous store has read it
-                __syncwarp();
-                if (a.residual)
+                if constexpr (SUM)
                 {
-                    const int64_t at = (int64_t)row0 * a.residual_ld + n;
-                    if (a.out_f32)
-                        global_to_box(box, static_cast<const float*>(a.residual) + at, a.residual_ld, live_rows,
-                                      live_cols, lane);
-                    else
-                        global_to_box(box, static_cast<const uint16_t*>(a.residual) + at, a.residual_ld, live_rows,
-                                      live_cols, lane);
-                    __syncwarp();
-                }
-            }
-            uint8_t* srow = box + lane * 128;
-#pragma unroll 1
-            for (int k = 0; k < box_cols / 32; k++)
-            {
-                uint32_t v[32];
-                tmem_ld32(t_row + c + 32 * k, v);
-                tmem_ld_wait();
-                float x[32];
-#pragma unroll
-                for (int j = 0; j < 32; j++) x[j] = __uint_as_float(v[j]);
-                if (bias) add_bias32(a, bias, n + 32 * k, x);
-                activate<32>(x, a.act);
-                if (gate) mul_gate32(a, gate, n + 32 * k, x);
-                if (a.out_f32)
-                {
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                    {
-                        float4* p = reinterpret_cast<float4*>(srow + ((j ^ sw) << 4));
-                        float4 o = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
-                        if (a.residual)
-                        {
-                            const float4 r = *p;
-                            o.x += r.x;
-                            o.y += r.y;
-                            o.z += r.z;
-                            o.w += r.w;
-                        }
-                        *p = o;
-                    }
+                    // no registers to spare: as it comes
+                    const float* p = static_cast<const float*>(a.residual) + (int64_t)row0 * a.residual_ld + un.n0 + c + lane;
+                    const bool in = un.n0 + c + lane < a.N;
+#pragma unroll 8
+                    for (int r = 0; r < live_rows; r++)
+                        if (in) *reinterpret_cast<float*>(box + box_at(r, lane * 4)) = p[r * a.residual_ld];
                 }
                 else
                 {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                    {
-                        uint4* p = reinterpret_cast<uint4*>(srow + (((4 * k + j) ^ sw) << 4));
-                        if (a.residual)
-                        {
-                            const uint4 r = *p;
-                            const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                            {
-                                const float2 f = unpack_bf16x2(rw[e]);
-                                x[8 * j + 2 * e] += f.x;
-                                x[8 * j + 2 * e + 1] += f.y;
-                            }
-                        }
-                        *p = make_uint4(pack_bf16x2(x[8 * j], x[8 * j + 1]), pack_bf16x2(x[8 * j + 2], x[8 * j + 3]),
-                                        pack_bf16x2(x[8 * j + 4], x[8 * j + 5]),
-                                        pack_bf16x2(x[8 * j + 6], x[8 * j + 7]));
-                    }
+                    next.put(a, box, lane);
+                    if (c + box_cols < c_hi && un.n0 + c + box_cols < a.N)
+                        next.load(a, row0, un.n0 + c + box_cols, live_rows, lane);
                 }
+                __syncwarp();
             }
+            return true;
+        };
+        auto close_box = [&](int c) {
+            uint8_t* box = stg + (q % R) * kBox;
+            const int n = un.n0 + c;
+            const int live_cols = min(box_cols, a.N - n);
             const bool whole = a.tma_out && live_rows == 32;
             fence_proxy_async_smem();
             __syncwarp();
@@ -405,19 +511,74 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
                     issue_load();        // box q+R-1 into it
                 }
             }
-        }
-        if (!ok) break;
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0)
+            q++;
+        };
+
+        if constexpr (SUM)
         {
-            if (CTAS == 2)
-                mbar_arrive_cluster(mapa_shared(&tempty[acc], 0));
-            else
-                mbar_arrive(&tempty[acc]);
+            float sum[COLS / 32][32];
+#pragma unroll
+            for (int i = 0; i < COLS / 32; i++)
+#pragma unroll
+                for (int j = 0; j < 32; j++) sum[i][j] = 0.f;
+            for (int kb = 0; kb < a.num_kb; kb += a.chunk_kb)
+            {
+                ok = wait_acc();
+                if (!ok) break;
+                const uint32_t t_row = t_lane + acc * BN + c_lo;
+#pragma unroll
+                for (int i = 0; i < COLS / 16; i++)
+                {
+                    uint32_t v[16];
+                    tmem_ld16(t_row + 16 * i, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; j++) sum[i / 2][16 * (i % 2) + j] += __uint_as_float(v[j]);
+                }
+                release_acc();
+            }
+            if (!ok) break;
+            // unrolled: `sum` stays in registers
+#pragma unroll
+            for (int i = 0; i < COLS / 32; i++)
+            {
+                const int c = c_lo + 32 * i;
+                if (un.n0 + c >= a.N || live_rows <= 0 || !ok) continue;
+                ok = open_box(c);
+                if (!ok) continue;
+                // sixteen columns at a time: no registers for more
+#pragma unroll
+                for (int j = 0; j < 32; j += 16)
+                    finish<16>(a, &sum[i][j], bias, gate, un.n0 + c + j, stg + (q % R) * kBox + lane * 128, sw, j);
+                close_box(c);
+            }
         }
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1;
+        else
+        {
+            ok = wait_acc();
+            if (!ok) break;
+            const uint32_t t_row = t_lane + acc * BN;
+#pragma unroll 1
+            for (int c = c_lo; c < c_hi && un.n0 + c < a.N && live_rows > 0; c += box_cols)
+            {
+                ok = open_box(c);
+                if (!ok) break;
+#pragma unroll 1
+                for (int k = 0; k < box_cols / 32; k++)
+                {
+                    uint32_t v[32];
+                    tmem_ld32(t_row + c + 32 * k, v);
+                    tmem_ld_wait();
+                    float x[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) x[j] = __uint_as_float(v[j]);
+                    finish<32>(a, x, bias, gate, un.n0 + c + 32 * k, stg + (q % R) * kBox + lane * 128, sw, 32 * k);
+                }
+                close_box(c);
+            }
+            if (!ok) break;
+            release_acc();
+        }
     }
     if (lane == 0)
     {
@@ -429,8 +590,8 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
     __syncwarp();
 }
 
-template <int CTAS, int BN, int R>
-__global__ void __launch_bounds__(kTileThreads, 1)
+template <int CTAS, int BN, int R, bool SUM>
+__global__ void __launch_bounds__(tile_threads(SUM), 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                        const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ CUtensorMap tmap_res,
                        const LinearArgs args)
@@ -497,6 +658,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int units = first[args.groups];
     UnitWalk<CTAS * BM, BN> walk{off, first};
 
+    // each role's code follows its own setmaxnreg, so that the compiler gives
+    // it that many registers
+    if (warp >= first_epilogue_warp(SUM))
+    {
+        if constexpr (SUM) regs_increase<kSumRegs>();
+        const int e = warp - first_epilogue_warp(SUM);
+        tile_epilogue<CTAS, BN, R, SUM>(args, &tmap_out, &tmap_res, walk, walk, unit0, step, units, rank,
+                                        epi_stage + e * R * kBox, rfull + e * R, tfull, tempty, tmem_base, warp & 3,
+                                        e >> 2, lane, abort_flag);
+    }
+    else
+    {
+    if constexpr (SUM) regs_decrease<kOtherRegs>();
     if (warp == 0)
     {
         if (lane == 0)
@@ -552,47 +726,50 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             uint32_t phase = 0, acc_phase = 0;
             for (int u = unit0; u < units && !*abort_flag; u += step)
             {
-                if (!mbar_wait<true>(&tempty[acc], acc_phase ^ 1, abort_flag, args.status)) break;
-                tc_fence_after();
-                const uint32_t d_tmem = tmem_base + acc * BN;
                 bool ok = true;
-                for (int kb = 0; kb < args.num_kb; kb++)
+                for (int kb0 = 0; kb0 < args.num_kb && ok; kb0 += args.chunk_kb)
                 {
-                    if (!mbar_wait<true>(&full[stage], phase, abort_flag, args.status))
-                    {
-                        ok = false;
-                        break;
-                    }
+                    ok = mbar_wait<true>(&tempty[acc], acc_phase ^ 1, abort_flag, args.status);
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a_addr = smem_u32(smem + stage * TL::STAGE_BYTES);
-                    const uint32_t b_addr = a_addr + A_BYTES;
+                    const uint32_t d_tmem = tmem_base + acc * BN;
+                    const int kb1 = min(args.num_kb, kb0 + args.chunk_kb);
+                    for (int kb = kb0; kb < kb1; kb++)
+                    {
+                        ok = mbar_wait<true>(&full[stage], phase, abort_flag, args.status);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t a_addr = smem_u32(smem + stage * TL::STAGE_BYTES);
+                        const uint32_t b_addr = a_addr + A_BYTES;
 #pragma unroll
-                    for (int k = 0; k < BK / 16; k++)
-                    {
-                        const uint64_t ad = umma_desc_sw128(a_addr + k * 32, 16, 1024);
-                        const uint64_t bd = umma_desc_sw128(b_addr + k * 32, 16, 1024);
+                        for (int k = 0; k < BK / 16; k++)
+                        {
+                            const uint64_t ad = umma_desc_sw128(a_addr + k * 32, 16, 1024);
+                            const uint64_t bd = umma_desc_sw128(b_addr + k * 32, 16, 1024);
+                            if (CTAS == 2)
+                                umma_bf16_pair(d_tmem, ad, bd, TL::IDESC, kb > kb0 || k > 0);
+                            else
+                                umma_bf16(d_tmem, ad, bd, TL::IDESC, kb > kb0 || k > 0);
+                        }
                         if (CTAS == 2)
-                            umma_bf16_pair(d_tmem, ad, bd, TL::IDESC, (kb | k) != 0);
+                            umma_commit_pair(&empty[stage], 0x3);
                         else
-                            umma_bf16(d_tmem, ad, bd, TL::IDESC, (kb | k) != 0);
+                            umma_commit(&empty[stage]);
+                        if (++stage == stages)
+                        {
+                            stage = 0;
+                            phase ^= 1;
+                        }
                     }
+                    if (!ok) break;
                     if (CTAS == 2)
-                        umma_commit_pair(&empty[stage], 0x3);
+                        umma_commit_pair(&tfull[acc], 0x3);
                     else
-                        umma_commit(&empty[stage]);
-                    if (++stage == stages)
-                    {
-                        stage = 0;
-                        phase ^= 1;
-                    }
+                        umma_commit(&tfull[acc]);
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1;
                 }
                 if (!ok) break;
-                if (CTAS == 2)
-                    umma_commit_pair(&tfull[acc], 0x3);
-                else
-                    umma_commit(&tfull[acc]);
-                acc ^= 1;
-                if (acc == 0) acc_phase ^= 1;
             }
             // every MMA completes (in both CTAs) before TMEM is released
             if (CTAS == 2)
@@ -602,12 +779,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         if (lane == 0) drain_wait(drain, 0);
     }
-    else
-    {
-        const int e = warp - 2;
-        tile_epilogue<CTAS, BN, R>(args, &tmap_out, &tmap_res, walk, walk, unit0, step, units, rank,
-                                   epi_stage + e * R * kBox, rfull + e * R, tfull, tempty, tmem_base, warp & 3, e >> 2,
-                                   lane, abort_flag);
     }
 
     tc_fence_before();
@@ -629,7 +800,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 // bound by reading W.  A cluster of S CTAs splits K; each leaves its fp32
 // partial sums in its shared memory, and after a cluster barrier CTA r adds
 // the S parts of rows r, r + S, ... in rank order (the result does not depend
-// on the run), applies the epilogue and stores.
+// on the run), applies the epilogue and stores: a warp takes one row's 128
+// features, four a lane.
 constexpr int kRowsThreads = 192;
 
 template <int TN>
@@ -643,28 +815,127 @@ struct RowsShape
     static constexpr int STAGES = (112 * 1024 - PART_BYTES - 1024 - 256) / STAGE_BYTES;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + PART_BYTES + 1024 + 256;
     static constexpr uint32_t IDESC = umma_idesc_bf16(128, TN, 0, 0);
-    static constexpr int TMEM_COLS = TN < 32 ? 32 : TN;
-    static_assert((2 * STAGES + 3) * 8 + 8 <= 256, "barriers");
+    static constexpr int ACC_COLS = TN < 32 ? 32 : TN;
+    static constexpr int TMEM_COLS = 2 * ACC_COLS; // two accumulators
+    static_assert((2 * STAGES + 5) * 8 + 8 <= 256, "barriers");
 };
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr)
 {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
     return v;
 }
 
-template <int TN>
+// Rows rank, rank + S, ... of the unit: the S parts added, the epilogue, the
+// store.  Two rows at once, so that 2 S loads are in flight.
+template <int S>
+__device__ __forceinline__ void rows_finish(const LinearArgs& a, const float* part, int rank, int warp, int lane,
+                                            int group, int64_t row0, int live, int n0)
+{
+    const int n = n0 + lane * 4;
+    if (n >= a.N) return;
+    const bool four = n + 4 <= a.N;
+    float b[4], g[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+    {
+        b[e] = a.bias && n + e < a.N ? __ldg(a.bias + (int64_t)group * a.N + n + e) : 0.f;
+        g[e] = a.gate && n + e < a.N ? __ldg(a.gate + (int64_t)group * a.N + n + e) : 1.f;
+    }
+    uint32_t at[S];
+#pragma unroll
+    for (int k = 0; k < S; k++) at[k] = S > 1 ? mapa_shared(part + lane * 4, k) : smem_u32(part + lane * 4);
+    for (int r = rank + S * warp; r < live; r += 8 * S)
+    {
+        float x[2][4] = {};
+        const int rows = r + 4 * S < live ? 2 : 1;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+        {
+            float4 v[S];
+            if (i < rows)
+#pragma unroll
+                for (int k = 0; k < S; k++) v[k] = ld_cluster_v4(at[k] + (r + 4 * S * i) * 512);
+            if (i < rows)
+#pragma unroll
+                for (int k = 0; k < S; k++)
+                {
+                    x[i][0] += v[k].x;
+                    x[i][1] += v[k].y;
+                    x[i][2] += v[k].z;
+                    x[i][3] += v[k].w;
+                }
+        }
+        for (int i = 0; i < rows; i++)
+        {
+            const int64_t row = row0 + r + 4 * S * i;
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = x[i][e] + b[e];
+            activate<4>(y, a.act);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] *= g[e];
+            if (a.out_f32)
+            {
+                float* o = static_cast<float*>(a.out) + row * a.out_ld + n;
+                if (a.residual)
+                {
+                    const float* p = static_cast<const float*>(a.residual) + row * a.residual_ld + n;
+                    if (four && a.vec_res)
+                    {
+                        const float4 q = *reinterpret_cast<const float4*>(p);
+                        y[0] += q.x, y[1] += q.y, y[2] += q.z, y[3] += q.w;
+                    }
+                    else
+                        for (int e = 0; e < 4; e++)
+                            if (n + e < a.N) y[e] += p[e];
+                }
+                if (four && a.vec_out)
+                    *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
+                else
+                    for (int e = 0; e < 4; e++)
+                        if (n + e < a.N) o[e] = y[e];
+            }
+            else
+            {
+                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + row * a.out_ld + n;
+                if (a.residual)
+                {
+                    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.residual) + row * a.residual_ld + n;
+                    if (four && a.vec_res)
+                    {
+                        const uint2 q = *reinterpret_cast<const uint2*>(p);
+                        const float2 lo = unpack_bf16x2(q.x), hi = unpack_bf16x2(q.y);
+                        y[0] += lo.x, y[1] += lo.y, y[2] += hi.x, y[3] += hi.y;
+                    }
+                    else
+                        for (int e = 0; e < 4; e++)
+                            if (n + e < a.N) y[e] += __bfloat162float(p[e]);
+                }
+                if (four && a.vec_out)
+                    *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+                else
+                    for (int e = 0; e < 4; e++)
+                        if (n + e < a.N) o[e] = __float2bfloat16_rn(y[e]);
+            }
+        }
+    }
+}
+
+template <int TN, int S>
 __global__ void __launch_bounds__(kRowsThreads, 2)
     linear_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                        const LinearArgs args)
 {
     using RS = RowsShape<TN>;
     constexpr int STAGES = RS::STAGES;
-    const int S = args.cluster;
     const int rank = S > 1 ? (int)cluster_ctarank() : 0;
     const int unit = blockIdx.x / S;
-    const int group = unit / args.nblk;
+    const int group = args.groups > 1 ? unit / args.nblk : 0;
     const int n0 = (unit - group * args.nblk) * 128;
     int lo = 0, hi = args.rows;
     if (args.offsets)
@@ -674,7 +945,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         hi = max(0, min(b, args.rows));
         if ((a != lo || b != hi || hi < lo) && threadIdx.x == 0) record_status(args.status, kStatusBadIndex);
     }
-    if (hi <= lo) return; // the whole cluster: no rows in this group
+    // row tiles blockIdx.y, + gridDim.y, ...: the same in every CTA of the cluster
+    const int tiles = hi > lo ? (hi - lo + TN - 1) / TN : 0;
+    if ((int)blockIdx.y >= tiles) return;
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -682,13 +955,32 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * RS::STAGE_BYTES + RS::PART_BYTES);
     uint64_t* empty = full + STAGES;
     uint64_t* tfull = empty + STAGES;
-    uint64_t* tempty = tfull + 1;
-    uint64_t* drain = tempty + 1;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* drain = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
+    const int kb0 = (int)((int64_t)args.num_kb * rank / S);
+    const int kb1 = (int)((int64_t)args.num_kb * (rank + 1) / S);
+
+    int stage = 0;
+    uint32_t phase = 0, issued = 0, last_phase = 0;
+    auto load = [&](int kb, int row0) {
+        uint8_t* sw = smem + stage * RS::STAGE_BYTES;
+        mbar_arrive_expect_tx(&full[stage], RS::STAGE_BYTES);
+        tma_load_2d(sw, &tmap_w, &full[stage], kb * BK, group * args.N + n0);
+        tma_load_2d(sw + RS::W_BYTES, &tmap_a, &full[stage], kb * BK, row0);
+        issued |= 1u << stage;
+        last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
+        if (++stage == STAGES)
+        {
+            stage = 0;
+            phase ^= 1;
+        }
+    };
+    int early = 0; // K blocks of the first row tile already sent for
     if (threadIdx.x == 0)
     {
         for (int s = 0; s < STAGES; s++)
@@ -696,14 +988,18 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        mbar_init(tfull, 1);
-        mbar_init(tempty, 4);
+        for (int b = 0; b < 2; b++)
+        {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], 4);
+        }
         mbar_init(drain, 1);
         *abort_flag = 0;
         *tmem_slot = 0;
         fence_mbarrier_init();
-        tma_prefetch_desc(&tmap_a);
-        tma_prefetch_desc(&tmap_w);
+        fence_proxy_async_smem();
+        // the ring's first fill does not wait for the set-up below
+        for (; early < STAGES && kb0 + early < kb1; early++) load(kb0 + early, lo + (int)blockIdx.y * TN);
     }
     __syncthreads();
     if (warp == 1) tmem_alloc(tmem_slot, RS::TMEM_COLS);
@@ -712,12 +1008,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    const int kb0 = (int)((int64_t)args.num_kb * rank / S);
-    const int kb1 = (int)((int64_t)args.num_kb * (rank + 1) / S);
-    const int tiles = (hi - lo + TN - 1) / TN; // the same in every CTA of the cluster
-    int stage = 0;
-    uint32_t phase = 0, issued = 0, last_phase = 0;
-    for (int t = 0; t < tiles; t++)
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int t = blockIdx.y; t < tiles; t += gridDim.y)
     {
         const int row0 = lo + t * TN;
         const int live = min(TN, hi - row0);
@@ -725,63 +1018,64 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         {
             if (lane == 0)
             {
-                for (int kb = kb0; kb < kb1; kb++)
+                for (int kb = kb0 + early; kb < kb1; kb++)
                 {
                     if (!mbar_wait<true>(&empty[stage], phase ^ 1, abort_flag, args.status)) break;
-                    uint8_t* sw = smem + stage * RS::STAGE_BYTES;
-                    mbar_arrive_expect_tx(&full[stage], RS::STAGE_BYTES);
-                    tma_load_2d(sw, &tmap_w, &full[stage], kb * BK, group * args.N + n0);
-                    tma_load_2d(sw + RS::W_BYTES, &tmap_a, &full[stage], kb * BK, row0);
-                    issued |= 1u << stage;
-                    last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
-                    if (++stage == STAGES)
-                    {
-                        stage = 0;
-                        phase ^= 1;
-                    }
+                    load(kb, row0);
                 }
+                early = 0;
             }
             __syncwarp();
         }
         else if (warp == 1)
         {
-            if (lane == 0 && mbar_wait<true>(tempty, (t & 1) ^ 1, abort_flag, args.status))
+            if (lane == 0)
             {
-                tc_fence_after();
                 bool ok = true;
-                for (int kb = kb0; kb < kb1 && ok; kb++)
+                for (int c0 = kb0; c0 < kb1 && ok; c0 += args.chunk_kb)
                 {
-                    ok = mbar_wait<true>(&full[stage], phase, abort_flag, args.status);
+                    ok = mbar_wait<true>(&tempty[acc], acc_phase ^ 1, abort_flag, args.status);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t w_addr = smem_u32(smem + stage * RS::STAGE_BYTES);
-#pragma unroll
-                    for (int k = 0; k < BK / 16; k++)
-                        umma_bf16(tmem_base, umma_desc_sw128(w_addr + k * 32, 16, 1024),
-                                  umma_desc_sw128(w_addr + RS::W_BYTES + k * 32, 16, 1024), RS::IDESC,
-                                  kb > kb0 || k > 0);
-                    umma_commit(&empty[stage]);
-                    if (++stage == STAGES)
+                    const int c1 = min(kb1, c0 + args.chunk_kb);
+                    for (int kb = c0; kb < c1; kb++)
                     {
-                        stage = 0;
-                        phase ^= 1;
+                        ok = mbar_wait<true>(&full[stage], phase, abort_flag, args.status);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t w_addr = smem_u32(smem + stage * RS::STAGE_BYTES);
+#pragma unroll
+                        for (int k = 0; k < BK / 16; k++)
+                            umma_bf16(tmem_base + acc * RS::ACC_COLS, umma_desc_sw128(w_addr + k * 32, 16, 1024),
+                                      umma_desc_sw128(w_addr + RS::W_BYTES + k * 32, 16, 1024), RS::IDESC,
+                                      kb > c0 || k > 0);
+                        umma_commit(&empty[stage]);
+                        if (++stage == STAGES)
+                        {
+                            stage = 0;
+                            phase ^= 1;
+                        }
                     }
+                    if (!ok) break;
+                    umma_commit(&tfull[acc]);
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1;
                 }
-                if (ok) umma_commit(tfull);
             }
             __syncwarp();
         }
         else
         {
-            int ok = 0;
-            if (lane == 0) ok = mbar_wait<true>(tfull, t & 1, abort_flag, args.status) ? 1 : 0;
-            ok = __shfl_sync(0xffffffffu, ok, 0);
-            if (ok)
+            const int f = (warp & 3) * 32 + lane;
+            for (int c0 = kb0; c0 < kb1; c0 += args.chunk_kb)
             {
+                int ok = 0;
+                if (lane == 0) ok = mbar_wait<true>(&tfull[acc], acc_phase, abort_flag, args.status) ? 1 : 0;
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
                 __syncwarp();
                 tc_fence_after();
-                const int f = (warp & 3) * 32 + lane;
-                const uint32_t t_row = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+                const uint32_t t_row = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * RS::ACC_COLS;
 #pragma unroll 1
                 for (int c = 0; c < live; c += 32)
                 {
@@ -789,56 +1083,31 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
                     tmem_ld32(t_row + c, v);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (c + j < live) part[(c + j) * 128 + f] = __uint_as_float(v[j]);
+                    for (int j = 0; j < (TN < 32 ? TN : 32); j++)
+                    {
+                        float* p = part + (c + j) * 128 + f; // this thread's own until the cluster meets
+                        *p = c0 > kb0 ? *p + __uint_as_float(v[j]) : __uint_as_float(v[j]);
+                    }
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(tempty);
+                if (lane == 0) mbar_arrive(&tempty[acc]);
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1;
             }
         }
         __syncwarp();
         if (S > 1)
             cluster_sync();
-        if (warp >= 2 && !*abort_flag)
-        {
-            const int f = (warp & 3) * 32 + lane;
-            const int n = n0 + f;
-            if (n < args.N)
-            {
-                const float b = args.bias ? __ldg(args.bias + (int64_t)group * args.N + n) : 0.f;
-                const float gt = args.gate ? __ldg(args.gate + (int64_t)group * args.N + n) : 1.f;
-                for (int r = rank; r < live; r += S)
-                {
-                    float x[1] = {0.f};
-                    if (S > 1)
-                    {
-                        for (int k = 0; k < S; k++) x[0] += ld_cluster_f32(mapa_shared(part + r * 128 + f, k));
-                    }
-                    else
-                        x[0] = part[r * 128 + f]; // this thread's own
-                    x[0] += b;
-                    activate<1>(x, args.act);
-                    x[0] *= gt;
-                    const int64_t row = row0 + r;
-                    if (args.out_f32)
-                    {
-                        if (args.residual)
-                            x[0] += static_cast<const float*>(args.residual)[row * args.residual_ld + n];
-                        static_cast<float*>(args.out)[row * args.out_ld + n] = x[0];
-                    }
-                    else
-                    {
-                        if (args.residual)
-                            x[0] += __bfloat162float(
-                                static_cast<const __nv_bfloat16*>(args.residual)[row * args.residual_ld + n]);
-                        static_cast<__nv_bfloat16*>(args.out)[row * args.out_ld + n] = __float2bfloat16_rn(x[0]);
-                    }
-                }
-            }
-        }
+        else
+            __syncthreads();
+        if (warp >= 2 && !*abort_flag) rows_finish<S>(args, part, rank, warp - 2, lane, group, row0, live, n0);
         __syncwarp();
-        if (S > 1) cluster_sync(); // the parts are read before the next rows' overwrite them, or the CTA exits
+        // the parts are read before the next rows' overwrite them, or the CTA exits
+        if (S > 1)
+            cluster_sync();
+        else
+            __syncthreads();
     }
     if (warp == 0 && lane == 0 && *abort_flag)
         for (int s = 0; s < STAGES; s++)
@@ -880,11 +1149,11 @@ struct Operands
     int64_t ldw;
 };
 
-template <int CTAS, int BN, int R>
-int launch_tiles(Context& ctx, const Operands& o, LinearArgs a)
+template <int CTAS, int BN, int R, bool SUM>
+int launch_tiles_as(Context& ctx, const Operands& o, LinearArgs a)
 {
     using TL = TileShape<CTAS, BN, R>;
-    auto kernel = linear_tile_kernel<CTAS, BN, R>;
+    auto kernel = linear_tile_kernel<CTAS, BN, R, SUM>;
     CUtensorMap ta, tw, to, tr;
     int r = make_tmap_bf16_2d(&ta, o.A, a.K, a.rows, (uint64_t)o.lda * 2, BK, BM);
     if (r == S2_OK)
@@ -899,6 +1168,7 @@ int launch_tiles(Context& ctx, const Operands& o, LinearArgs a)
     a.nblk = (a.N + BN - 1) / BN;
     a.stages = TL::stages(a.groups);
     a.group_m = a.K >= 8192 ? 1 : (a.N <= 4096 ? 8 : 16);
+    a.chunk_kb = SUM ? kChunk : a.num_kb;
     const int64_t units = ((int64_t)a.rows / (CTAS * BM) + a.groups) * a.nblk; // at most
     if (units > 0x7fffffff) return S2_ERR_INVALID;
     const size_t smem = TL::fixed_bytes(a.groups) + (size_t)a.stages * TL::STAGE_BYTES;
@@ -907,11 +1177,15 @@ int launch_tiles(Context& ctx, const Operands& o, LinearArgs a)
     static std::atomic<int> resident{0};        // CTAs or pairs at once, the same on every B200
     if (first_on_device(configured))
     {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit) != cudaSuccess)
+        cudaFuncAttributes f;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit) != cudaSuccess ||
+            cudaFuncGetAttributes(&f, kernel) != cudaSuccess)
             return S2_ERR_CUDA;
+        // launched with fewer registers, setmaxnreg.inc would wait for good
+        if (SUM && f.numRegs != kLaunchRegs) return S2_ERR_CUDA;
     }
     cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = cluster_config(attr, CTAS, CTAS, kTileThreads, smem, ctx.stream);
+    cudaLaunchConfig_t cfg = cluster_config(attr, CTAS, CTAS, tile_threads(SUM), smem, ctx.stream);
     int most = CTAS == 1 ? ctx.num_sms : resident.load();
     if (most == 0)
     {
@@ -932,23 +1206,23 @@ int launch_tiles(Context& ctx, const Operands& o, LinearArgs a)
     return S2_OK;
 }
 
-template <int TN>
-int launch_rows(Context& ctx, const Operands& o, LinearArgs a)
+template <int CTAS, int BN, int R>
+int launch_tiles(Context& ctx, const Operands& o, const LinearArgs& a)
+{
+    return a.out_f32 && a.num_kb > kLongK ? launch_tiles_as<CTAS, BN, R, true>(ctx, o, a)
+                                          : launch_tiles_as<CTAS, BN, R, false>(ctx, o, a);
+}
+
+template <int TN, int S>
+int launch_rows_as(Context& ctx, const Operands& o, const LinearArgs& a, int row_tiles)
 {
     using RS = RowsShape<TN>;
-    auto kernel = linear_rows_kernel<TN>;
+    auto kernel = linear_rows_kernel<TN, S>;
     CUtensorMap ta, tw;
     int r = make_tmap_bf16_2d(&ta, o.A, a.K, a.rows, (uint64_t)o.lda * 2, BK, TN);
     if (r == S2_OK)
         r = make_tmap_bf16_2d(&tw, o.W, a.K, (uint64_t)a.groups * a.N, (uint64_t)o.ldw * 2, BK, 128);
     if (r != S2_OK) return r;
-    a.nblk = (a.N + 127) / 128;
-    const int64_t units = (int64_t)a.groups * a.nblk;
-    // K parts: as many as the two CTAs a SM leave room for
-    int s = 1;
-    while (s < 8 && 2 * s <= a.num_kb && units * 2 * s <= 2 * ctx.num_sms) s *= 2;
-    if (units * s > 0x7fffffff) return S2_ERR_INVALID;
-    a.cluster = s;
     static std::atomic<uint64_t> configured{0};
     if (first_on_device(configured))
     {
@@ -956,8 +1230,9 @@ int launch_rows(Context& ctx, const Operands& o, LinearArgs a)
             return S2_ERR_CUDA;
     }
     cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg =
-        cluster_config(attr, s, (unsigned)(units * s), kRowsThreads, RS::SMEM_BYTES, ctx.stream);
+    cudaLaunchConfig_t cfg = cluster_config(attr, S, (unsigned)(a.groups * a.nblk * S), kRowsThreads, RS::SMEM_BYTES,
+                                            ctx.stream);
+    cfg.gridDim.y = row_tiles;
     if (cudaLaunchKernelEx(&cfg, kernel, ta, tw, a) != cudaSuccess)
     {
         (void)cudaGetLastError();
@@ -965,6 +1240,35 @@ int launch_rows(Context& ctx, const Operands& o, LinearArgs a)
     }
     ctx.launches++;
     return S2_OK;
+}
+
+template <int TN>
+int launch_rows(Context& ctx, const Operands& o, LinearArgs a)
+{
+    a.nblk = (a.N + 127) / 128;
+    const int mean_rows = (a.rows + a.groups - 1) / a.groups;
+    const int row_tiles = std::min(65535, (mean_rows + TN - 1) / TN);
+    const int64_t units = (int64_t)a.groups * a.nblk * row_tiles;
+    // K parts: as many as the resident CTAs leave room for
+    const int room = 2 * ctx.num_sms;
+    int s = 1;
+    for (int p : {2, 3, 4, 6, 8})
+        if (p <= a.num_kb && units * p <= room) s = p;
+    if ((int64_t)a.groups * a.nblk * s > 0x7fffffff) return S2_ERR_INVALID;
+    a.cluster = s;
+    a.chunk_kb = a.out_f32 && a.num_kb > kLongK ? kChunk : a.num_kb;
+    const int esz = a.out_f32 ? 4 : 2;
+    a.vec_out = reinterpret_cast<uintptr_t>(a.out) % (4 * esz) == 0 && a.out_ld % 4 == 0;
+    a.vec_res = reinterpret_cast<uintptr_t>(a.residual) % (4 * esz) == 0 && a.residual_ld % 4 == 0;
+    switch (s)
+    {
+    case 1: return launch_rows_as<TN, 1>(ctx, o, a, row_tiles);
+    case 2: return launch_rows_as<TN, 2>(ctx, o, a, row_tiles);
+    case 3: return launch_rows_as<TN, 3>(ctx, o, a, row_tiles);
+    case 4: return launch_rows_as<TN, 4>(ctx, o, a, row_tiles);
+    case 6: return launch_rows_as<TN, 6>(ctx, o, a, row_tiles);
+    default: return launch_rows_as<TN, 8>(ctx, o, a, row_tiles);
+    }
 }
 
 int run_linear(s2_context* ctx, int rows, int groups, const int* offsets, int N, int K, const void* A, int64_t lda,
@@ -1009,11 +1313,31 @@ int run_linear(s2_context* ctx, int rows, int groups, const int* offsets, int N,
     ProfileScope prof(c, K_GEMM, 2.0 * rows * N * K,
                       ((double)rows * K + (double)groups * N * K) * 2.0 + (double)rows * N * osz);
     const int mean_rows = (rows + groups - 1) / groups;
-    if (mean_rows <= 16) return launch_rows<16>(c, o, a);
-    if (mean_rows <= 32) return launch_rows<32>(c, o, a);
-    if (mean_rows <= 64) return launch_rows<64>(c, o, a);
-    const int64_t pair_tiles = ((int64_t)rows / 256 + 1) * ((N + 255) / 256);
-    if (N > 128 && pair_tiles >= c.num_sms / 2) return launch_tiles<2, 256, 2>(c, o, a);
+    auto tiles = [&](int m, int n) { return (int64_t)groups * ((mean_rows + m - 1) / m) * ((N + n - 1) / n); };
+    // Few rows a group, or too few 128 x 128 tiles for half the SMs: the
+    // transposed product, whose K is split over clusters (2,560 x 2,560, 58
+    // rows: 13.3 us against 27.8 in tiles; 300 rows: 15.7 against 19.0; 512
+    // rows, 80 tiles: 22.6 against 19.9).
+    if (mean_rows <= 64 || tiles(128, 128) < c.num_sms / 2)
+    {
+        if (mean_rows <= 16) return launch_rows<16>(c, o, a);
+        if (mean_rows <= 32) return launch_rows<32>(c, o, a);
+        return launch_rows<64>(c, o, a);
+    }
+    // A round of 256 x 256 tiles on CTA pairs takes 1.45 times one of 128 x 128
+    // tiles for four times the work on twice the SMs, and wins unless its last
+    // round is mostly empty (2,560 x 2,560, 512 rows: 23.9 against 19.9 us;
+    // 1,000 rows: 25.8 against 31.7).
+    auto rounds = [&](int64_t t, int slots) { return (double)((t + slots - 1) / slots); };
+    if (N > 128 && 1.45 * rounds(tiles(256, 256), c.num_sms / 2) <= rounds(tiles(128, 128), c.num_sms))
+    {
+        // Boxes per epilogue warp: a third one costs an operand stage and pays
+        // where the epilogue moves a quarter of the operands' bytes or more
+        // (288,000 x 256 x 512 with a bf16 residual 109.7 against 116.4 us;
+        // 21,658 x 2,560 x 1,280: 119 against 116).
+        const double moved = 128.0 * 256 * osz, fed = (double)a.num_kb * 32768;
+        return moved >= 0.25 * fed ? launch_tiles<2, 256, 3>(c, o, a) : launch_tiles<2, 256, 2>(c, o, a);
+    }
     return launch_tiles<1, 128, 3>(c, o, a);
 }
 
