@@ -6,6 +6,7 @@
 //   * linear_rows_kernel: 128 output features a CTA against a few rows, K
 //     split over a thread-block cluster, for few rows a group.
 #include <algorithm>
+#include <cmath>
 
 #include "activation.cuh"
 #include "s2_common.cuh"
@@ -174,21 +175,24 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity)
 }
 
 // ---------------------------------------------------------------- many rows
-// Warps: TMA, MMA, then eight for the epilogue, two per TMEM lane quarter with
-// half the columns each.  Where these hold sums of the accumulator in registers
-// (SUM) they begin at warp 4, so that setmaxnreg can give them what the first
-// four do not need: 104 + 2 x 200 = 3 x 168 registers per thread and warpgroup,
-// the 168 a thread that 384 threads are launched with.
-constexpr int kEpiWarps = 8;
+// Warps: TMA, MMA, then EW for the epilogue, in equal parts over the four TMEM
+// lane quarters, each with its share of the columns.  Eight do where boxes
+// leave by TMA; sixteen where the warps copy them, a chain of latencies that
+// only more warps hide (21,247 x 409 x 303 in 56 groups, bf16 with a residual:
+// 44 us against 85; but 117 against 110 where TMA does it: 288,000 x 256 x 512).
+// Where a warp holds sums of the accumulator in registers (SUM) the eight begin
+// at warp 4, so that setmaxnreg can give them what the first four do not need:
+// 104 + 2 x 200 = 3 x 168 registers per thread and warpgroup, the 168 a thread
+// that 384 threads are launched with.
 constexpr int kSumRegs = 200, kOtherRegs = 104, kLaunchRegs = 168;
 static_assert(kOtherRegs + 2 * kSumRegs == 3 * kLaunchRegs, "register split");
 constexpr int first_epilogue_warp(bool sum)
 {
     return sum ? 4 : 2;
 }
-constexpr int tile_threads(bool sum)
+constexpr int tile_threads(int EW, bool sum)
 {
-    return 32 * (first_epilogue_warp(sum) + kEpiWarps);
+    return 32 * (first_epilogue_warp(sum) + EW);
 }
 template <int N>
 __device__ __forceinline__ void regs_increase()
@@ -204,12 +208,13 @@ constexpr int kBox = 4096; // 32 rows x 128 bytes
 
 // CTAS = 2: a pair of CTAs (cluster of 2) computes 256 rows x BN columns with
 // M = 256 MMAs, each holding its 128 rows of A and BN / 2 rows of W.
-template <int CTAS, int BN, int R>
+// R: boxes per epilogue warp.
+template <int CTAS, int BN, int R, int EW>
 struct TileShape
 {
     static constexpr int W_BYTES = BN / CTAS * BK * 2;
     static constexpr int STAGE_BYTES = A_BYTES + W_BYTES;
-    static constexpr int EPI_BYTES = kEpiWarps * R * kBox;
+    static constexpr int EPI_BYTES = EW * R * kBox;
     static constexpr int TMEM_COLS = 2 * BN;
     static constexpr uint32_t IDESC = umma_idesc_bf16(CTAS * BM, BN, 0, 0);
     static constexpr int MAX_STAGES = 8;
@@ -238,57 +243,130 @@ __device__ __forceinline__ int box_at(int r, int b)
 }
 
 // Rows and columns that a tensor map cannot take (group ends inside a box,
-// strides or bases off 16 bytes): the warp copies element by element.
-template <typename T>
-__device__ __forceinline__ void box_to_global(const uint8_t* box, T* out, int64_t ld, int rows, int cols, int lane)
+// strides or bases off 16 bytes): the warp copies row by row, a 32-bit word a
+// lane.  A bf16 row that begins off a word is shifted by one element between
+// the lanes, and its first and last elements go by themselves.
+__device__ __forceinline__ uint32_t box_word(const uint8_t* box, int r, int lane)
 {
-    constexpr int W = 128 / sizeof(T);
-#pragma unroll 8
-    for (int r = 0; r < rows; r++)
-#pragma unroll
-        for (int c = lane; c < W; c += 32)
-            if (c < cols) out[r * ld + c] = *reinterpret_cast<const T*>(box + box_at(r, c * (int)sizeof(T)));
+    return *reinterpret_cast<const uint32_t*>(box + box_at(r, lane * 4));
+}
+// Predicated accesses: written as branches, the three a bf16 row needs took
+// 6,000 cycles a box instead of some 1,500.
+__device__ __forceinline__ void st32_if(bool p, void* to, uint32_t v)
+{
+    asm volatile("{.reg .pred p; setp.ne.b32 p, %2, 0; @p st.global.b32 [%0], %1;}" ::"l"(to), "r"(v), "r"((int)p)
+                 : "memory");
+}
+__device__ __forceinline__ void st16_if(bool p, void* to, uint32_t v)
+{
+    asm volatile("{.reg .pred p; setp.ne.b32 p, %2, 0; @p st.global.b16 [%0], %1;}" ::"l"(to), "h"((uint16_t)v),
+                 "r"((int)p)
+                 : "memory");
+}
+// 0 where p is false
+__device__ __forceinline__ uint32_t ld32_if(bool p, const void* from)
+{
+    uint32_t v;
+    asm volatile("{.reg .pred p; setp.ne.b32 p, %2, 0; mov.b32 %0, 0; @p ld.global.b32 %0, [%1];}"
+                 : "=r"(v)
+                 : "l"(from), "r"((int)p)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t ld16_if(bool p, const void* from)
+{
+    uint16_t v;
+    asm volatile("{.reg .pred p; setp.ne.b32 p, %2, 0; mov.b16 %0, 0; @p ld.global.b16 %0, [%1];}"
+                 : "=h"(v)
+                 : "l"(from), "r"((int)p)
+                 : "memory");
+    return v;
 }
 
-// A residual box in registers, one word a row (fp32: column `lane`; bf16:
-// columns `lane` and `lane + 32`), so that all of it is in flight at once.
-struct HeldBox
+__device__ __forceinline__ void box_to_global(const uint8_t* box, float* out, int64_t ld, int rows, int cols, int lane)
 {
-    uint32_t w[32];
-    __device__ void load(const LinearArgs& a, int row0, int n, int rows, int lane)
+    constexpr int B = 8;
+    out += lane;
+    for (int r0 = 0; r0 < rows; r0 += B)
     {
-        const int64_t ld = a.residual_ld;
-        if (a.out_f32)
-        {
-            const uint32_t* p = static_cast<const uint32_t*>(a.residual) + (int64_t)row0 * ld + n + lane;
+        uint32_t w[B];
 #pragma unroll
-            for (int r = 0; r < 32; r++) w[r] = r < rows && n + lane < a.N ? p[r * ld] : 0u;
-        }
-        else
-        {
-            const uint16_t* p = static_cast<const uint16_t*>(a.residual) + (int64_t)row0 * ld + n + lane;
+        for (int i = 0; i < B; i++) w[i] = box_word(box, r0 + i, lane);
 #pragma unroll
-            for (int r = 0; r < 32; r++)
-            {
-                const uint32_t lo = r < rows && n + lane < a.N ? p[r * ld] : 0u;
-                const uint32_t hi = r < rows && n + lane + 32 < a.N ? p[r * ld + 32] : 0u;
-                w[r] = lo | hi << 16;
-            }
+        for (int i = 0; i < B; i++, out += ld) st32_if(lane < cols && r0 + i < rows, out, w[i]);
+    }
+}
+__device__ __forceinline__ void box_to_global(const uint8_t* box, uint16_t* out, int64_t ld, int rows, int cols, int lane)
+{
+    constexpr int B = 8;
+    cols = min(cols, 64);
+    for (int r0 = 0; r0 < rows; r0 += B)
+    {
+        uint32_t w[B];
+#pragma unroll
+        for (int i = 0; i < B; i++) w[i] = box_word(box, r0 + i, lane);
+#pragma unroll
+        for (int i = 0; i < B; i++, out += ld)
+        {
+            const uint32_t next = __shfl_down_sync(0xffffffffu, w[i], 1);
+            const int off = (reinterpret_cast<uintptr_t>(out) >> 1) & 1;
+            const uint32_t v = __byte_perm(w[i], next, off ? 0x5432 : 0x3210);
+            const int e = 2 * lane + off; // the word's first element
+            const bool in = r0 + i < rows;
+            st32_if(in && e + 1 < cols, out + e, v);
+            st16_if(in && e + 1 == cols, out + e, v);
+            st16_if(in && off && lane == 0, out, w[i]);
         }
     }
-    __device__ void put(const LinearArgs& a, uint8_t* box, int lane) const
+}
+
+// Residual rows -> the box.
+__device__ __forceinline__ void global_to_box(uint8_t* box, const float* in, int64_t ld, int rows, int cols, int lane)
+{
+    constexpr int B = 16;
+    in += lane;
+    for (int r0 = 0; r0 < rows; r0 += B)
     {
+        uint32_t w[B];
 #pragma unroll
-        for (int r = 0; r < 32; r++)
-            if (a.out_f32)
-                *reinterpret_cast<uint32_t*>(box + box_at(r, lane * 4)) = w[r];
-            else
-            {
-                *reinterpret_cast<uint16_t*>(box + box_at(r, lane * 2)) = (uint16_t)w[r];
-                *reinterpret_cast<uint16_t*>(box + box_at(r, lane * 2 + 64)) = (uint16_t)(w[r] >> 16);
-            }
+        for (int i = 0; i < B; i++, in += ld) w[i] = ld32_if(lane < cols && r0 + i < rows, in);
+#pragma unroll
+        for (int i = 0; i < B; i++) *reinterpret_cast<uint32_t*>(box + box_at(r0 + i, lane * 4)) = w[i];
     }
-};
+}
+__device__ __forceinline__ void global_to_box(uint8_t* box, const uint16_t* in, int64_t ld, int rows, int cols, int lane)
+{
+    constexpr int B = 8;
+    cols = min(cols, 64);
+    for (int r0 = 0; r0 < rows; r0 += B)
+    {
+        uint32_t w[B], one[B]; // one: a last odd element, or (lane 0) the first of a row off a word
+        const uint16_t* row = in;
+#pragma unroll
+        for (int i = 0; i < B; i++, row += ld)
+        {
+            const int off = (reinterpret_cast<uintptr_t>(row) >> 1) & 1;
+            const int e = 2 * lane + off;
+            const bool live = r0 + i < rows;
+            w[i] = ld32_if(live && e + 1 < cols, row + e);
+            w[i] |= ld16_if(live && e + 1 == cols, row + e);
+            one[i] = ld16_if(live && off && lane == 0, row);
+        }
+#pragma unroll
+        for (int i = 0; i < B; i++, in += ld)
+        {
+            const uint32_t before = __shfl_up_sync(0xffffffffu, w[i], 1);
+            const int off = (reinterpret_cast<uintptr_t>(in) >> 1) & 1;
+            const uint32_t shifted = (lane == 0 ? one[i] : before >> 16) | w[i] << 16;
+            *reinterpret_cast<uint32_t*>(box + box_at(r0 + i, lane * 4)) = off ? shifted : w[i];
+        }
+    }
+}
+__device__ __forceinline__ void prefetch_row(const void* from, const void* to)
+{
+    for (uintptr_t p = reinterpret_cast<uintptr_t>(from) & ~uintptr_t(127); p < reinterpret_cast<uintptr_t>(to); p += 128)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
 
 // W accumulator columns of this lane's row -> the result, in the box (srow: the
 // lane's row of it; col: the first column's place in the box).
@@ -357,23 +435,27 @@ __device__ __forceinline__ void finish(const LinearArgs& a, const float* x0, con
 // Epilogue of one warp over all of the CTA's units.  Boxes (32 rows x 128
 // bytes of output) run in a fixed sequence; each is combined in one of the
 // warp's R shared-memory boxes and written by one TMA store.  A residual box is
-// TMA-loaded R - 1 boxes ahead into the slot its result will leave from, or
-// held in registers one box ahead where TMA cannot take it.  SUM (fp32 results,
+// TMA-loaded R - 1 boxes ahead (R = 1: as soon as the box before has left) into
+// the slot its result will leave from; where
+// TMA cannot take it the warp copies it.  Either way a unit's residual is asked
+// for in L2 a unit ahead.  SUM (fp32 results,
 // long K): the accumulator's chunks are added up in registers first.
-template <int CTAS, int BN, int R, bool SUM>
+template <int CTAS, int BN, int R, int EW, bool SUM>
 __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtensorMap* tmap_out,
                                               const CUtensorMap* tmap_res, UnitWalk<CTAS * BM, BN> walk,
                                               UnitWalk<CTAS * BM, BN> ahead, int first_unit, int step, int units,
                                               int rank, uint8_t* stg, uint64_t* rfull, uint64_t* tfull,
-                                              uint64_t* tempty, uint32_t tmem_base, int quarter, int half, int lane,
+                                              uint64_t* tempty, uint32_t tmem_base, int quarter, int part, int lane,
                                               volatile int* abort_flag)
 {
-    constexpr int COLS = BN / 2; // of a unit, per warp
-    const int box_cols = SUM ? 32 : (a.out_f32 ? 32 : 64);
+    constexpr int COLS = BN * 4 / EW; // of a unit, per warp
+    constexpr int PIECE = EW > 8 ? 16 : 32; // columns at a time: by the registers there are
+    const int esz = SUM || a.out_f32 ? 4 : 2;
+    const int box_cols = 128 / esz;
     const int row_in = rank * BM + quarter * 32; // of the unit, this warp's first
-    const int c_lo = half * COLS, c_hi = c_lo + COLS;
+    const int c_lo = part * COLS, c_hi = c_lo + COLS;
     const int sw = lane & 7;
-    const bool held = a.residual && !a.tma_res;
+    const bool copied = a.residual && !a.tma_res;
     // loader cursor (lane 0)
     int lu = first_unit, lc = c_lo, lq = 0;
     Unit lun{};
@@ -398,20 +480,26 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
         lq++;
         lc += box_cols;
     };
-    // a unit's residual boxes go to L2 a unit ahead
+    // a unit's residual goes to L2 a unit ahead
     UnitWalk<CTAS * BM, BN> far = ahead;
     auto prefetch_unit = [&](int u) {
-        if (u >= units) return;
+        if (!a.residual || u >= units) return;
         const Unit p = far.decode(a, u);
-        if (p.m0 + row_in >= p.end) return;
-        for (int c = c_lo; c < c_hi && p.n0 + c < a.N; c += box_cols)
-            tma_prefetch_l2_2d(tmap_res, p.n0 + c, p.m0 + row_in);
+        const int row = p.m0 + row_in;
+        if (a.tma_res)
+        {
+            if (lane == 0 && row < p.end)
+                for (int c = c_lo; c < c_hi && p.n0 + c < a.N; c += box_cols) tma_prefetch_l2_2d(tmap_res, p.n0 + c, row);
+        }
+        else if (row + lane < p.end && p.n0 + c_lo < a.N)
+        {
+            const uint8_t* line = static_cast<const uint8_t*>(a.residual) + (int64_t)(row + lane) * a.residual_ld * esz;
+            prefetch_row(line + (int64_t)(p.n0 + c_lo) * esz, line + (int64_t)min(p.n0 + c_hi, a.N) * esz);
+        }
     };
+    prefetch_unit(first_unit);
     if (a.tma_res && lane == 0)
-    {
-        prefetch_unit(first_unit);
-        for (int i = 0; i < R - 1; i++) issue_load();
-    }
+        for (int i = 0; i < (R > 1 ? R - 1 : 1); i++) issue_load();
 
     int q = 0, acc = 0;
     uint32_t acc_phase = 0;
@@ -445,9 +533,7 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
         const float* bias = a.bias ? a.bias + (int64_t)un.group * a.N : nullptr;
         const float* gate = a.gate ? a.gate + (int64_t)un.group * a.N : nullptr;
         const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
-        if (a.tma_res && lane == 0) prefetch_unit(u + step);
-        HeldBox next;
-        if (!SUM && held && live_rows > 0 && un.n0 + c_lo < a.N) next.load(a, row0, un.n0 + c_lo, live_rows, lane);
+        prefetch_unit(u + step);
 
         // box q of the warp, columns [c, c + box_cols) of the unit: from its
         // slot's release to its store
@@ -463,23 +549,14 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
             }
             if (lane == 0) bulk_wait_read<R - 1>(); // this slot's previous store has read it
             __syncwarp();
-            if (held)
+            if (copied)
             {
-                if constexpr (SUM)
-                {
-                    // no registers to spare: as it comes
-                    const float* p = static_cast<const float*>(a.residual) + (int64_t)row0 * a.residual_ld + un.n0 + c + lane;
-                    const bool in = un.n0 + c + lane < a.N;
-#pragma unroll 8
-                    for (int r = 0; r < live_rows; r++)
-                        if (in) *reinterpret_cast<float*>(box + box_at(r, lane * 4)) = p[r * a.residual_ld];
-                }
+                const int64_t at = (int64_t)row0 * a.residual_ld + un.n0 + c;
+                const int cols = a.N - un.n0 - c;
+                if (esz == 4)
+                    global_to_box(box, static_cast<const float*>(a.residual) + at, a.residual_ld, live_rows, cols, lane);
                 else
-                {
-                    next.put(a, box, lane);
-                    if (c + box_cols < c_hi && un.n0 + c + box_cols < a.N)
-                        next.load(a, row0, un.n0 + c + box_cols, live_rows, lane);
-                }
+                    global_to_box(box, static_cast<const uint16_t*>(a.residual) + at, a.residual_ld, live_rows, cols, lane);
                 __syncwarp();
             }
             return true;
@@ -507,8 +584,10 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
                 bulk_commit();
                 if (a.tma_res)
                 {
-                    bulk_wait_read<1>(); // the store of box q-1 has read box (q-1) % R
-                    issue_load();        // box q+R-1 into it
+                    // the store of box q-1 (of q itself if there is but one) has
+                    // read its slot, which takes the next load
+                    bulk_wait_read<(R > 1 ? 1 : 0)>();
+                    issue_load();
                 }
             }
             q++;
@@ -564,15 +643,18 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
                 ok = open_box(c);
                 if (!ok) break;
 #pragma unroll 1
-                for (int k = 0; k < box_cols / 32; k++)
+                for (int k = 0; k < box_cols; k += PIECE)
                 {
-                    uint32_t v[32];
-                    tmem_ld32(t_row + c + 32 * k, v);
+                    uint32_t v[PIECE];
+                    if constexpr (PIECE == 32)
+                        tmem_ld32(t_row + c + k, v);
+                    else
+                        tmem_ld16(t_row + c + k, v);
                     tmem_ld_wait();
-                    float x[32];
+                    float x[PIECE];
 #pragma unroll
-                    for (int j = 0; j < 32; j++) x[j] = __uint_as_float(v[j]);
-                    finish<32>(a, x, bias, gate, un.n0 + c + 32 * k, stg + (q % R) * kBox + lane * 128, sw, 32 * k);
+                    for (int j = 0; j < PIECE; j++) x[j] = __uint_as_float(v[j]);
+                    finish<PIECE>(a, x, bias, gate, un.n0 + c + k, stg + (q % R) * kBox + lane * 128, sw, k);
                 }
                 close_box(c);
             }
@@ -590,13 +672,13 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
     __syncwarp();
 }
 
-template <int CTAS, int BN, int R, bool SUM>
-__global__ void __launch_bounds__(tile_threads(SUM), 1)
+template <int CTAS, int BN, int R, int EW, bool SUM>
+__global__ void __launch_bounds__(tile_threads(EW, SUM), 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                        const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ CUtensorMap tmap_res,
                        const LinearArgs args)
 {
-    using TL = TileShape<CTAS, BN, R>;
+    using TL = TileShape<CTAS, BN, R, EW>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int stages = args.stages;
@@ -606,10 +688,10 @@ __global__ void __launch_bounds__(tile_threads(SUM), 1)
     uint64_t* tfull = empty + TL::MAX_STAGES;
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
-    uint64_t* rfull = drain + 1; // [kEpiWarps][R]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + kEpiWarps * R);
+    uint64_t* rfull = drain + 1; // [EW][R]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + EW * R);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((2 * TL::MAX_STAGES + 5 + kEpiWarps * R) * 8 + 8 <= 512, "barriers");
+    static_assert((2 * TL::MAX_STAGES + 5 + EW * R) * 8 + 8 <= 512, "barriers");
     int* off = reinterpret_cast<int*>(epi_stage + TL::EPI_BYTES + 512);
     int* first = off + args.groups + 1;
 
@@ -629,10 +711,10 @@ __global__ void __launch_bounds__(tile_threads(SUM), 1)
         for (int b = 0; b < 2; b++)
         {
             mbar_init(&tfull[b], 1);
-            mbar_init(&tempty[b], CTAS * kEpiWarps);
+            mbar_init(&tempty[b], CTAS * EW);
         }
         mbar_init(drain, 1);
-        for (int i = 0; i < kEpiWarps * R; i++) mbar_init(&rfull[i], 1);
+        for (int i = 0; i < EW * R; i++) mbar_init(&rfull[i], 1);
         *abort_flag = 0;
         *tmem_slot = 0;
         fence_mbarrier_init();
@@ -664,7 +746,7 @@ __global__ void __launch_bounds__(tile_threads(SUM), 1)
     {
         if constexpr (SUM) regs_increase<kSumRegs>();
         const int e = warp - first_epilogue_warp(SUM);
-        tile_epilogue<CTAS, BN, R, SUM>(args, &tmap_out, &tmap_res, walk, walk, unit0, step, units, rank,
+        tile_epilogue<CTAS, BN, R, EW, SUM>(args, &tmap_out, &tmap_res, walk, walk, unit0, step, units, rank,
                                         epi_stage + e * R * kBox, rfull + e * R, tfull, tempty, tmem_base, warp & 3,
                                         e >> 2, lane, abort_flag);
     }
@@ -1149,22 +1231,22 @@ struct Operands
     int64_t ldw;
 };
 
-template <int CTAS, int BN, int R, bool SUM>
-int launch_tiles_as(Context& ctx, const Operands& o, LinearArgs a)
+// Output and residual maps, where TMA can take them.
+struct BoxMaps
 {
-    using TL = TileShape<CTAS, BN, R>;
-    auto kernel = linear_tile_kernel<CTAS, BN, R, SUM>;
-    CUtensorMap ta, tw, to, tr;
+    CUtensorMap out, res;
+};
+
+template <int CTAS, int BN, int R, int EW, bool SUM>
+int launch_tiles(Context& ctx, const Operands& o, const BoxMaps& m, LinearArgs a)
+{
+    using TL = TileShape<CTAS, BN, R, EW>;
+    auto kernel = linear_tile_kernel<CTAS, BN, R, EW, SUM>;
+    CUtensorMap ta, tw;
     int r = make_tmap_bf16_2d(&ta, o.A, a.K, a.rows, (uint64_t)o.lda * 2, BK, BM);
     if (r == S2_OK)
         r = make_tmap_bf16_2d(&tw, o.W, a.K, (uint64_t)a.groups * a.N, (uint64_t)o.ldw * 2, BK, BN / CTAS);
     if (r != S2_OK) return r;
-    const int esz = a.out_f32 ? 4 : 2;
-    a.tma_out = make_tmap_2d(&to, a.out, a.out_f32, a.N, a.rows, (uint64_t)a.out_ld * esz, 128 / esz, 32) == S2_OK;
-    if (!a.tma_out) to = ta;
-    a.tma_res = a.residual && make_tmap_2d(&tr, a.residual, a.out_f32, a.N, a.rows, (uint64_t)a.residual_ld * esz,
-                                           128 / esz, 32) == S2_OK;
-    if (!a.tma_res) tr = ta;
     a.nblk = (a.N + BN - 1) / BN;
     a.stages = TL::stages(a.groups);
     a.group_m = a.K >= 8192 ? 1 : (a.N <= 4096 ? 8 : 16);
@@ -1185,7 +1267,7 @@ int launch_tiles_as(Context& ctx, const Operands& o, LinearArgs a)
         if (SUM && f.numRegs != kLaunchRegs) return S2_ERR_CUDA;
     }
     cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = cluster_config(attr, CTAS, CTAS, tile_threads(SUM), smem, ctx.stream);
+    cudaLaunchConfig_t cfg = cluster_config(attr, CTAS, CTAS, tile_threads(EW, SUM), smem, ctx.stream);
     int most = CTAS == 1 ? ctx.num_sms : resident.load();
     if (most == 0)
     {
@@ -1197,20 +1279,13 @@ int launch_tiles_as(Context& ctx, const Operands& o, LinearArgs a)
         resident.store(most);
     }
     cfg.gridDim = dim3((unsigned)(CTAS * std::min<int64_t>(units, most)));
-    if (cudaLaunchKernelEx(&cfg, kernel, ta, tw, to, tr, a) != cudaSuccess)
+    if (cudaLaunchKernelEx(&cfg, kernel, ta, tw, a.tma_out ? m.out : ta, a.tma_res ? m.res : ta, a) != cudaSuccess)
     {
         (void)cudaGetLastError();
         return S2_ERR_CUDA;
     }
     ctx.launches++;
     return S2_OK;
-}
-
-template <int CTAS, int BN, int R>
-int launch_tiles(Context& ctx, const Operands& o, const LinearArgs& a)
-{
-    return a.out_f32 && a.num_kb > kLongK ? launch_tiles_as<CTAS, BN, R, true>(ctx, o, a)
-                                          : launch_tiles_as<CTAS, BN, R, false>(ctx, o, a);
 }
 
 template <int TN, int S>
@@ -1313,7 +1388,12 @@ int run_linear(s2_context* ctx, int rows, int groups, const int* offsets, int N,
     ProfileScope prof(c, K_GEMM, 2.0 * rows * N * K,
                       ((double)rows * K + (double)groups * N * K) * 2.0 + (double)rows * N * osz);
     const int mean_rows = (rows + groups - 1) / groups;
-    auto tiles = [&](int m, int n) { return (int64_t)groups * ((mean_rows + m - 1) / m) * ((N + n - 1) / n); };
+    // Tiles of m x n; the sizes of several groups are not known here: each ends
+    // in half a tile on average.
+    auto tiles = [&](int m, int n) {
+        const double row_tiles = groups == 1 ? (rows + m - 1) / m : groups * ((double)rows / groups / m + 0.5);
+        return row_tiles * ((N + n - 1) / n);
+    };
     // Few rows a group, or too few 128 x 128 tiles for half the SMs: the
     // transposed product, whose K is split over clusters (2,560 x 2,560, 58
     // rows: 13.3 us against 27.8 in tiles; 300 rows: 15.7 against 19.0; 512
@@ -1328,17 +1408,30 @@ int run_linear(s2_context* ctx, int rows, int groups, const int* offsets, int N,
     // tiles for four times the work on twice the SMs, and wins unless its last
     // round is mostly empty (2,560 x 2,560, 512 rows: 23.9 against 19.9 us;
     // 1,000 rows: 25.8 against 31.7).
-    auto rounds = [&](int64_t t, int slots) { return (double)((t + slots - 1) / slots); };
-    if (N > 128 && 1.45 * rounds(tiles(256, 256), c.num_sms / 2) <= rounds(tiles(128, 128), c.num_sms))
+    auto rounds = [&](double t, int slots) { return std::ceil(t / slots); };
+    const bool pair = N > 128 && 1.45 * rounds(tiles(256, 256), c.num_sms / 2) <= rounds(tiles(128, 128), c.num_sms);
+    BoxMaps m;
+    const int esz = a.out_f32 ? 4 : 2;
+    a.tma_out = make_tmap_2d(&m.out, out, a.out_f32, N, rows, (uint64_t)ldo * esz, 128 / esz, 32) == S2_OK;
+    a.tma_res = a.residual && make_tmap_2d(&m.res, a.residual, a.out_f32, N, rows, (uint64_t)a.residual_ld * esz,
+                                           128 / esz, 32) == S2_OK;
+    // Boxes per epilogue warp: a third one costs an operand stage and pays
+    // where the epilogue moves much beside the operands (of 128 x 256 outputs a
+    // CTA): from a quarter of their bytes on (288,000 x 256 x 512 with a bf16
+    // residual 111 against 116 us; 21,658 x 2,560 x 1,280: 119 against 116),
+    // for sums from a fifth (21,658 x 2,560 x 2,560 with an fp32 residual 265
+    // against 281 us; x 10,240: 869 against 847).
+    const double moved = 128.0 * 256 * osz, fed = (double)a.num_kb * 32768;
+    if (a.out_f32 && a.num_kb > kLongK)
     {
-        // Boxes per epilogue warp: a third one costs an operand stage and pays
-        // where the epilogue moves a quarter of the operands' bytes or more
-        // (288,000 x 256 x 512 with a bf16 residual 109.7 against 116.4 us;
-        // 21,658 x 2,560 x 1,280: 119 against 116).
-        const double moved = 128.0 * 256 * osz, fed = (double)a.num_kb * 32768;
-        return moved >= 0.25 * fed ? launch_tiles<2, 256, 3>(c, o, a) : launch_tiles<2, 256, 2>(c, o, a);
+        if (!pair) return launch_tiles<1, 128, 2, 8, true>(c, o, m, a);
+        return moved >= 0.2 * fed ? launch_tiles<2, 256, 3, 8, true>(c, o, m, a)
+                                  : launch_tiles<2, 256, 2, 8, true>(c, o, m, a);
     }
-    return launch_tiles<1, 128, 3>(c, o, a);
+    if (!pair) return launch_tiles<1, 128, 2, 8, false>(c, o, m, a);
+    if (!a.tma_out || (a.residual && !a.tma_res)) return launch_tiles<2, 256, 1, 16, false>(c, o, m, a);
+    return moved >= 0.25 * fed ? launch_tiles<2, 256, 3, 8, false>(c, o, m, a)
+                               : launch_tiles<2, 256, 2, 8, false>(c, o, m, a);
 }
 
 } // namespace
