@@ -912,12 +912,71 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr)
     return v;
 }
 
+// Four residuals of a row from column n on, as they lie in memory.
+struct Res4
+{
+    float v[4];
+    __device__ void load(const LinearArgs& a, int64_t row, int n, bool four)
+    {
+        if (a.out_f32)
+        {
+            const float* p = static_cast<const float*>(a.residual) + row * a.residual_ld + n;
+            if (four && a.vec_res)
+            {
+                const float4 q = *reinterpret_cast<const float4*>(p);
+                v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+            }
+            else
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = __uint_as_float(ld32_if(n + e < a.N, p + e));
+        }
+        else
+        {
+            const uint16_t* p = static_cast<const uint16_t*>(a.residual) + row * a.residual_ld + n;
+            if (four && a.vec_res)
+            {
+                const uint2 q = *reinterpret_cast<const uint2*>(p);
+                const float2 lo = unpack_bf16x2(q.x), hi = unpack_bf16x2(q.y);
+                v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
+            }
+            else
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = __uint_as_float(ld16_if(n + e < a.N, p + e) << 16);
+        }
+    }
+};
+
+__device__ __forceinline__ void store4(const LinearArgs& a, int64_t row, int n, bool four, const float (&y)[4])
+{
+    if (a.out_f32)
+    {
+        float* o = static_cast<float*>(a.out) + row * a.out_ld + n;
+        if (four && a.vec_out)
+            *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; e++) st32_if(n + e < a.N, o + e, __float_as_uint(y[e]));
+    }
+    else
+    {
+        uint16_t* o = static_cast<uint16_t*>(a.out) + row * a.out_ld + n;
+        const uint32_t lo = pack_bf16x2(y[0], y[1]), hi = pack_bf16x2(y[2], y[3]);
+        if (four && a.vec_out)
+            *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; e++) st16_if(n + e < a.N, o + e, (e < 2 ? lo : hi) >> 16 * (e & 1));
+    }
+}
+
 // Rows rank, rank + S, ... of the unit: the S parts added, the epilogue, the
-// store.  Two rows at once, so that 2 S loads are in flight.
+// store.  Several rows at once, their loads first, so that these are in flight
+// together.
 template <int S>
 __device__ __forceinline__ void rows_finish(const LinearArgs& a, const float* part, int rank, int warp, int lane,
                                             int group, int64_t row0, int live, int n0)
 {
+    constexpr int B = S > 4 ? 2 : 4; // rows at once
     const int n = n0 + lane * 4;
     if (n >= a.N) return;
     const bool four = n + 4 <= a.N;
@@ -931,79 +990,41 @@ __device__ __forceinline__ void rows_finish(const LinearArgs& a, const float* pa
     uint32_t at[S];
 #pragma unroll
     for (int k = 0; k < S; k++) at[k] = S > 1 ? mapa_shared(part + lane * 4, k) : smem_u32(part + lane * 4);
-    for (int r = rank + S * warp; r < live; r += 8 * S)
+    for (int r = rank + S * warp; r < live; r += 4 * S * B)
     {
-        float x[2][4] = {};
-        const int rows = r + 4 * S < live ? 2 : 1;
+        Res4 res[B];
+        float x[B][4] = {};
+        if (a.residual)
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+            for (int i = 0; i < B; i++)
+                if (r + 4 * S * i < live) res[i].load(a, row0 + r + 4 * S * i, n, four);
+#pragma unroll
+        for (int i = 0; i < B; i++)
         {
+            const int rr = min(r + 4 * S * i, live - 1); // a row past the end is read again and not used
             float4 v[S];
-            if (i < rows)
 #pragma unroll
-                for (int k = 0; k < S; k++) v[k] = ld_cluster_v4(at[k] + (r + 4 * S * i) * 512);
-            if (i < rows)
+            for (int k = 0; k < S; k++) v[k] = ld_cluster_v4(at[k] + rr * 512);
 #pragma unroll
-                for (int k = 0; k < S; k++)
-                {
-                    x[i][0] += v[k].x;
-                    x[i][1] += v[k].y;
-                    x[i][2] += v[k].z;
-                    x[i][3] += v[k].w;
-                }
+            for (int k = 0; k < S; k++)
+            {
+                x[i][0] += v[k].x;
+                x[i][1] += v[k].y;
+                x[i][2] += v[k].z;
+                x[i][3] += v[k].w;
+            }
         }
-        for (int i = 0; i < rows; i++)
+#pragma unroll
+        for (int i = 0; i < B; i++)
         {
-            const int64_t row = row0 + r + 4 * S * i;
+            if (r + 4 * S * i >= live) break;
             float y[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = x[i][e] + b[e];
             activate<4>(y, a.act);
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] *= g[e];
-            if (a.out_f32)
-            {
-                float* o = static_cast<float*>(a.out) + row * a.out_ld + n;
-                if (a.residual)
-                {
-                    const float* p = static_cast<const float*>(a.residual) + row * a.residual_ld + n;
-                    if (four && a.vec_res)
-                    {
-                        const float4 q = *reinterpret_cast<const float4*>(p);
-                        y[0] += q.x, y[1] += q.y, y[2] += q.z, y[3] += q.w;
-                    }
-                    else
-                        for (int e = 0; e < 4; e++)
-                            if (n + e < a.N) y[e] += p[e];
-                }
-                if (four && a.vec_out)
-                    *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
-                else
-                    for (int e = 0; e < 4; e++)
-                        if (n + e < a.N) o[e] = y[e];
-            }
-            else
-            {
-                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + row * a.out_ld + n;
-                if (a.residual)
-                {
-                    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.residual) + row * a.residual_ld + n;
-                    if (four && a.vec_res)
-                    {
-                        const uint2 q = *reinterpret_cast<const uint2*>(p);
-                        const float2 lo = unpack_bf16x2(q.x), hi = unpack_bf16x2(q.y);
-                        y[0] += lo.x, y[1] += lo.y, y[2] += hi.x, y[3] += hi.y;
-                    }
-                    else
-                        for (int e = 0; e < 4; e++)
-                            if (n + e < a.N) y[e] += __bfloat162float(p[e]);
-                }
-                if (four && a.vec_out)
-                    *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
-                else
-                    for (int e = 0; e < 4; e++)
-                        if (n + e < a.N) o[e] = __float2bfloat16_rn(y[e]);
-            }
+            for (int e = 0; e < 4; e++) y[e] = a.residual ? fmaf(y[e], g[e], res[i].v[e]) : y[e] * g[e];
+            store4(a, row0 + r + 4 * S * i, n, four, y);
         }
     }
 }
@@ -1322,13 +1343,16 @@ int launch_rows(Context& ctx, const Operands& o, LinearArgs a)
 {
     a.nblk = (a.N + 127) / 128;
     const int mean_rows = (a.rows + a.groups - 1) / a.groups;
-    const int row_tiles = std::min(65535, (mean_rows + TN - 1) / TN);
-    const int64_t units = (int64_t)a.groups * a.nblk * row_tiles;
-    // K parts: as many as the resident CTAs leave room for
+    int row_tiles = std::min(65535, (mean_rows + TN - 1) / TN);
+    const int64_t units = (int64_t)a.groups * a.nblk;
+    // K parts: as many as the resident CTAs leave room for; then, for groups of
+    // unknown sizes, CTAs for the row tiles of larger ones (without rows they
+    // return at once; otherwise one CTA takes a group's tiles in turn)
     const int room = 2 * ctx.num_sms;
     int s = 1;
     for (int p : {2, 3, 4, 6, 8})
-        if (p <= a.num_kb && units * p <= room) s = p;
+        if (p <= a.num_kb && units * row_tiles * p <= room) s = p;
+    if (a.groups > 1 && mean_rows > 8) row_tiles = std::max(row_tiles, 4);
     if ((int64_t)a.groups * a.nblk * s > 0x7fffffff) return S2_ERR_INVALID;
     a.cluster = s;
     a.chunk_kb = a.out_f32 && a.num_kb > kLongK ? kChunk : a.num_kb;
@@ -1394,21 +1418,27 @@ int run_linear(s2_context* ctx, int rows, int groups, const int* offsets, int N,
         const double row_tiles = groups == 1 ? (rows + m - 1) / m : groups * ((double)rows / groups / m + 0.5);
         return row_tiles * ((N + n - 1) / n);
     };
-    // Few rows a group, or too few 128 x 128 tiles for half the SMs: the
-    // transposed product, whose K is split over clusters (2,560 x 2,560, 58
-    // rows: 13.3 us against 27.8 in tiles; 300 rows: 15.7 against 19.0; 512
-    // rows, 80 tiles: 22.6 against 19.9).
-    if (mean_rows <= 64 || tiles(128, 128) < c.num_sms / 2)
+    // The transposed product, whose K is split over clusters: up to 8 rows a
+    // group (64 groups of 2,048 x 1,024 at 2 rows 37 us, against 44 in tiles;
+    // at 10 rows 61 against 49), up to 64 where the tiles are few (2,560 x
+    // 2,560, 64 rows 9.6 us against 16.7; 16 groups of 2,048 x 2,048 at 19 rows
+    // 24 against 29; 32 of 1,024 x 2,048 at 31 rows, 256 tiles, 35 against 33),
+    // and more rows of one group while half the SMs would have no tile (2,560 x
+    // 2,560: 300 rows 14.2 us against 17.8; 512 rows, 80 tiles, 19.8 against 17.9).
+    const double few = tiles(128, 128);
+    if (mean_rows <= 8 || (mean_rows <= 64 && few < 1.2 * c.num_sms) || (groups == 1 && few < 0.5 * c.num_sms))
     {
-        if (mean_rows <= 16) return launch_rows<16>(c, o, a);
-        if (mean_rows <= 32) return launch_rows<32>(c, o, a);
+        // groups somewhat above the mean still fit one row tile
+        const int most = groups == 1 ? rows : mean_rows + mean_rows / 2;
+        if (most <= 16) return launch_rows<16>(c, o, a);
+        if (most <= 32) return launch_rows<32>(c, o, a);
         return launch_rows<64>(c, o, a);
     }
     // A round of 256 x 256 tiles on CTA pairs takes 1.45 times one of 128 x 128
     // tiles for four times the work on twice the SMs, and wins unless its last
     // round is mostly empty (2,560 x 2,560, 512 rows: 23.9 against 19.9 us;
     // 1,000 rows: 25.8 against 31.7).
-    auto rounds = [&](double t, int slots) { return std::ceil(t / slots); };
+    auto rounds = [&](double t, int slots) { return groups == 1 ? std::ceil(t / slots) : t / slots + 0.5; };
     const bool pair = N > 128 && 1.45 * rounds(tiles(256, 256), c.num_sms / 2) <= rounds(tiles(128, 128), c.num_sms);
     BoxMaps m;
     const int esz = a.out_f32 ? 4 : 2;
