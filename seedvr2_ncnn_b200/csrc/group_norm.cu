@@ -74,6 +74,11 @@ struct Raw<float, 4>
 {
     uint4 q;
 };
+template <>
+struct Raw<__nv_bfloat16, 4>
+{
+    uint2 q;
+};
 
 // As pairs; V = 1 leaves the second half of its pair zero.
 template <int V>
@@ -89,6 +94,8 @@ __device__ __forceinline__ void unpack(const Raw<T, V>& r, float2 (&f)[kPairs<V>
 {
     if constexpr (V == 8)
         f[0] = bf16_pair(r.q.x), f[1] = bf16_pair(r.q.y), f[2] = bf16_pair(r.q.z), f[3] = bf16_pair(r.q.w);
+    else if constexpr (V == 4 && sizeof(T) == 2)
+        f[0] = bf16_pair(r.q.x), f[1] = bf16_pair(r.q.y);
     else if constexpr (V == 4)
     {
         f[0] = make_float2(__uint_as_float(r.q.x), __uint_as_float(r.q.y));
@@ -103,7 +110,7 @@ __device__ __forceinline__ Raw<T, V> load_raw(const T* p)
 {
     Raw<T, V> r;
     if constexpr (V > 1)
-        r.q = __ldcs(reinterpret_cast<const uint4*>(p));
+        r.q = __ldcs(reinterpret_cast<const decltype(r.q)*>(p));
     else
         r.v[0] = *p;
     return r;
@@ -160,6 +167,7 @@ __device__ __forceinline__ void join_groups(int first, int count, int slots, int
         // around the first entry's mean, so that a mean far from zero loses nothing
         const float p = live > 0 ? get(g, 0, 0).y : 0.f;
         float n = 0.f, s = 0.f;
+#pragma unroll 4
         for (int sl = s0; sl < live; sl += s_step)
             for (int u = u0; u < units; u += 1 << log_u)
             {
@@ -453,25 +461,31 @@ __global__ void __launch_bounds__(kThreads, 1) group_norm_slab_kernel(const Grou
 }
 
 // ---------------------------------------------------------------- sums, apply
-// Rows of a thread's column in order.  16-byte vectors come through a private
+// Rows of a thread's column in order.  Vectors come through a private
 // ring of shared memory filled by cp.async: no barrier, since a thread reads
 // only what it fetched itself, and no registers held while a row is on its
 // way.  kStep rows are fetched and handed out together, kDepth - 1 such steps
 // ahead; begin() sends for the first of them.  Single channels are loaded
-// plainly.
+// plainly, kPlain rows at once.
 constexpr int kDepth = 4;
 constexpr int kStep = 4;
-template <int V>
-constexpr size_t kRingBytes = V > 1 ? (size_t)kThreads * 16 * kStep * kDepth : 0;
+constexpr int kPlain = 8;
+template <typename TI, int V>
+constexpr size_t kRingBytes = V > 1 ? (size_t)kThreads * sizeof(Raw<TI, V>) * kStep * kDepth : 0;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src)
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src)
 {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 
 template <typename TI, int V>
 struct RowStream
 {
+    static constexpr int VB = sizeof(Raw<TI, V>), ROW = kThreads * VB;
     const TI* next;
     int64_t step;
     int n, unfetched;
@@ -479,17 +493,17 @@ struct RowStream
 
     __device__ void fetch(int slot)
     {
-        const uint32_t to = smem_u32(mine) + slot * (kStep * kThreads * 16);
+        const uint32_t to = smem_u32(mine) + slot * (kStep * ROW);
         if (unfetched >= kStep)
         {
 #pragma unroll
-            for (int u = 0; u < kStep; u++) cp_async16(to + u * (kThreads * 16), next + u * step);
+            for (int u = 0; u < kStep; u++) cp_async<VB>(to + u * ROW, next + u * step);
         }
         else
         {
 #pragma unroll
             for (int u = 0; u < kStep - 1; u++)
-                if (u < unfetched) cp_async16(to + u * (kThreads * 16), next + u * step);
+                if (u < unfetched) cp_async<VB>(to + u * ROW, next + u * step);
         }
         unfetched -= kStep;
         next += kStep * step;
@@ -500,7 +514,7 @@ struct RowStream
         next = x;
         step = step_;
         n = unfetched = n_;
-        mine = ring + threadIdx.x * 16;
+        mine = ring + threadIdx.x * VB;
         if constexpr (V > 1)
         {
 #pragma unroll
@@ -521,13 +535,13 @@ struct RowStream
                     if (left <= 0) break;
                     asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
                     Raw<TI, V> r;
-                    const uint8_t* at = mine + d * (kStep * kThreads * 16);
+                    const uint8_t* at = mine + d * (kStep * ROW);
                     if (left >= kStep)
                     {
 #pragma unroll
                         for (int u = 0; u < kStep; u++)
                         {
-                            r.q = *reinterpret_cast<const uint4*>(at + u * (kThreads * 16));
+                            r.q = *reinterpret_cast<const decltype(r.q)*>(at + u * ROW);
                             f(r);
                         }
                     }
@@ -536,7 +550,7 @@ struct RowStream
 #pragma unroll 1
                         for (int u = 0; u < left; u++)
                         {
-                            r.q = *reinterpret_cast<const uint4*>(at + u * (kThreads * 16));
+                            r.q = *reinterpret_cast<const decltype(r.q)*>(at + u * ROW);
                             f(r);
                         }
                     }
@@ -547,7 +561,18 @@ struct RowStream
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         else
-            for (int k = 0; k < n; k++, next += step) f(load_raw<TI, V>(next));
+        {
+            int k = 0;
+            for (; k + kPlain <= n; k += kPlain, next += kPlain * step)
+            {
+                Raw<TI, V> r[kPlain];
+#pragma unroll
+                for (int u = 0; u < kPlain; u++) r[u] = load_raw<TI, V>(next + u * step);
+#pragma unroll
+                for (int u = 0; u < kPlain; u++) f(r[u]);
+            }
+            for (; k < n; k++, next += step) f(load_raw<TI, V>(next));
+        }
     }
 };
 
@@ -720,8 +745,8 @@ struct Cut
     int slice, parts;
 };
 
-// How a problem is cut for vectors of V channels (16 bytes, or 1 where groups,
-// strides or bases do not admit 16-byte accesses).
+// How a problem is cut for vectors of V channels (16 or 8 bytes, or 1 where
+// groups, strides or bases do not admit them).
 //   Slab kernel: slices of 64 bytes (more CTAs; 256 x 512 bf16 4.7 us, against
 //   5.0 in slices of 128 bytes and 5.5 with clusters of 8), clusters as small
 //   as hold the rows, and only where all of it is resident at once (two CTAs a
@@ -745,8 +770,10 @@ Cut cut(int64_t instances, int64_t rows, int C, int width, int V)
     }
     if (!c.slab)
     {
-        const int u8 = width / gcd(width, 8) * 8; // the same slices for every V
-        c.slice = widest_slice(C, C % u8 == 0 ? u8 : width, 128);
+        // the same slices for every V that vectors_fit() admits: multiples of 8
+        // channels where these fit the row, else of 4, else single groups
+        const int u8 = width / gcd(width, 8) * 8, u4 = width / gcd(width, 4) * 4;
+        c.slice = widest_slice(C, C % u8 == 0 ? u8 : (C % u4 == 0 ? u4 : width), 128);
         const int64_t runs = instances * (C / c.slice);
         c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kPartCtas / runs, (rows + 31) / 32));
     }
@@ -820,21 +847,28 @@ int launch(Context& ctx, GroupNormArgs a, int instances, int C, void* workspace)
     a.partial = static_cast<float2*>(workspace);
     static std::atomic<uint64_t> seen_sums{0}, seen_apply{0};
     const int r = launch_kernel(ctx, group_norm_sums_kernel<TI, V>, seen_sums, grid, 1,
-                                (size_t)a.groups * 16 + (size_t)kThreads * (V / a.sub) * 8 + kRingBytes<V>, false, a);
+                                (size_t)a.groups * 16 + (size_t)kThreads * (V / a.sub) * 8 + kRingBytes<TI, V>, false, a);
     if (r != S2_OK) return r;
-    return launch_kernel(ctx, group_norm_apply_kernel<TI, TO, V>, seen_apply, grid, 1, ((size_t)a.groups * 8 + 15) / 16 * 16 + kRingBytes<V>, true, a);
+    return launch_kernel(ctx, group_norm_apply_kernel<TI, TO, V>, seen_apply, grid, 1, ((size_t)a.groups * 8 + 15) / 16 * 16 + kRingBytes<TI, V>, true, a);
+}
+
+// Vectors of V channels: whole ones in a row's groups, at aligned addresses.
+template <typename TI, typename TO, int V>
+bool vectors_fit(const GroupNormArgs& a, int C)
+{
+    const int unit = a.width / gcd(a.width, V) * V;
+    const size_t in = V * sizeof(TI), out = std::min<size_t>(16, V * sizeof(TO));
+    return C % unit == 0 && (a.ldx * sizeof(TI)) % in == 0 && (a.ldo * sizeof(TO)) % out == 0 &&
+           reinterpret_cast<uintptr_t>(a.x) % in == 0 && reinterpret_cast<uintptr_t>(a.out) % out == 0;
 }
 
 template <typename TI, typename TO>
 int launch_types(Context& ctx, const GroupNormArgs& a, int instances, int C, void* ws)
 {
-    // 16 bytes a thread where rows and groups allow it
-    constexpr int V = 16 / sizeof(TI);
-    const int unit = a.width / gcd(a.width, V) * V;
-    const bool vec = C % unit == 0 && (a.ldx * (int64_t)sizeof(TI)) % 16 == 0 && (a.ldo * (int64_t)sizeof(TO)) % 16 == 0 &&
-                     (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-    return vec ? launch<TI, TO, V>(ctx, a, instances, C, ws)
-               : launch<TI, TO, 1>(ctx, a, instances, C, ws);
+    if constexpr (sizeof(TI) == 2)
+        if (vectors_fit<TI, TO, 8>(a, C)) return launch<TI, TO, 8>(ctx, a, instances, C, ws);
+    if (vectors_fit<TI, TO, 4>(a, C)) return launch<TI, TO, 4>(ctx, a, instances, C, ws);
+    return launch<TI, TO, 1>(ctx, a, instances, C, ws);
 }
 
 } // namespace

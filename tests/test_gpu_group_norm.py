@@ -30,7 +30,8 @@ def _affine(seed, c):
 SIZES = [(1, 1, 8, 1), (1, 1, 64, 8), (2, 2, 32, 32), (1, 256, 512, 32), (3, 7, 320, 32), (3, 1185, 320, 32),
          (2, 100, 7, 7), (2, 333, 30, 3), (1, 50, 1000, 1), (2, 65, 2048, 1), (1, 40, 4104, 1), (24, 5, 96, 32),
          (1, 20000, 64, 32), (5, 3600, 256, 32), (1, 3000, 1536, 32), (40, 17, 128, 8), (1, 9, 2047, 23),
-         (2, 19, 4096, 4096)]
+         (2, 19, 4096, 4096), (2, 3000, 660, 20), (40, 100, 660, 20), (3, 2500, 20, 5), (9, 4000, 39, 1),
+         (300, 7, 12, 3), (5, 1200, 1980, 60)]
 
 
 @pytest.mark.parametrize("size", SIZES, ids=str)
