@@ -502,42 +502,43 @@ def _new(ctx, shape, code):
                        dtype=torch.float32 if code == S2_DTYPE_F32 else torch.bfloat16)
 
 
-def _operand(t, dim: int, device: int, what: str) -> int:
+def _operand_stride(t, device: int, what: str) -> int:
     """Row stride of a bf16 operand; a single row, which has none of its own, gets its length rounded up to 8."""
-    _require(t.dim() == dim and _dtype_code(t, what) == S2_DTYPE_BF16 and t.get_device() == device, what)
-    ld = _row_stride(t, what)
+    _require(_dtype_code(t, what) == S2_DTYPE_BF16 and t.get_device() == device, what)
     k = t.shape[-1]
-    return (k + 7) // 8 * 8 if t.numel() == k else ld
+    return (k + 7) // 8 * 8 if t.numel() == k else _row_stride(t, what)
 
 
 def _linear(ctx, what, a, weight, offsets, bias, act, gate, residual, out_dtype, out):
     dev = ctx.device
+    a_shape, w_shape = a.shape, weight.shape
     grouped = offsets is not None
-    lda, ldw = _operand(a, 2, dev, what), _operand(weight, 3 if grouped else 2, dev, what)
-    rows, K = a.shape
-    N = weight.shape[-2]
-    _require(weight.shape[-1] == K, what)
-    groups = weight.shape[0] if grouped else 1
+    _require(len(a_shape) == 2 and len(w_shape) == (3 if grouped else 2) and w_shape[-1] == a_shape[1], what)
+    rows, K = a_shape
+    N = w_shape[-2]
+    lda, ldw = _operand_stride(a, dev, what), _operand_stride(weight, dev, what)
     if out is None:
         out = _new(ctx, (rows, N), out_dtype)
     code = _dtype_code(out, what)
     _require(out.shape == (rows, N) and out.get_device() == dev, what)
-    vec = (groups, N) if grouped else (N,)
+    vec = w_shape[:-1]  # (N,), or (groups, N)
     e = LinearEpilogue(act, _vector(bias, vec, dev, what), _vector(gate, vec, dev, what), None, 0)
     if residual is not None:
         _require(residual.dtype == out.dtype and residual.shape == out.shape and residual.get_device() == dev, what)
         e.residual = residual.data_ptr()
         e.residual_ld = _row_stride(residual, what)
-    L = lib()
+    ldo = N if out.is_contiguous() else _row_stride(out, what)
     if grouped:
-        _require(str(offsets.dtype) == "torch.int32" and offsets.shape == (groups + 1,) and offsets.is_contiguous()
-                 and offsets.get_device() == dev, what)
-        r = L.s2_grouped_linear(ctx.handle, rows, groups, offsets.data_ptr(), N, K, a.data_ptr(), lda,
-                                weight.data_ptr(), ldw, C.byref(e), code, out.data_ptr(), _row_stride(out, what))
+        groups = w_shape[0]
+        _require(offsets.element_size() == 4 and not offsets.is_floating_point() and offsets.shape == (groups + 1,)
+                 and offsets.is_contiguous() and offsets.get_device() == dev, what)
+        r = lib().s2_grouped_linear(ctx.handle, rows, groups, offsets.data_ptr(), N, K, a.data_ptr(), lda,
+                                    weight.data_ptr(), ldw, C.byref(e), code, out.data_ptr(), ldo)
     else:
-        r = L.s2_linear(ctx.handle, rows, N, K, a.data_ptr(), lda, weight.data_ptr(), ldw, C.byref(e), code,
-                        out.data_ptr(), _row_stride(out, what))
-    check(r, what)
+        r = lib().s2_linear(ctx.handle, rows, N, K, a.data_ptr(), lda, weight.data_ptr(), ldw, C.byref(e), code,
+                            out.data_ptr(), ldo)
+    if r:
+        check(r, what)
     return out
 
 
@@ -579,8 +580,7 @@ def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=
         import torch
 
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        if ctx.stream != torch.cuda.current_stream(dev):
-            ws.record_stream(ctx.stream)
+        ws.record_stream(ctx.stream)  # freed here, used there
     vec = (channels,)
     check(L.s2_group_norm(ctx.handle, instances, rows, channels, groups, code, x.data_ptr(), _row_stride(x, what),
                           _vector(gamma, vec, dev, what), _vector(beta, vec, dev, what), eps, act, out_code,

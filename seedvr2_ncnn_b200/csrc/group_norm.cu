@@ -53,6 +53,7 @@ struct GroupNormArgs
     int part_rows, longer; // the first `longer` parts have part_rows + 1 rows, the others part_rows
     uint32_t by_width;     // c / width = umulhi(c, by_width) for width > 1 and c * width < 2^32
     int sub;         // channels of one group that lie in one thread's vector
+    int red_bytes;   // of the sums kernel's reduction, before its ring
     float eps;
     int act;
     float2* partial; // [instances][slices * groups][parts] (mean, M2)
@@ -202,7 +203,7 @@ __device__ __forceinline__ float3 join2(float3 a, float3 b)
 // Sums around p of n values in each of V channels -> (mean, M2), `sub`
 // consecutive channels of one group joined: V / sub entries of `red`.
 template <int V, int SUB>
-__device__ __forceinline__ void merge_channels(const float (&m)[V], const float (&q)[V], float n, float2* red)
+__device__ __forceinline__ void merge_channels(const float (&m)[V], const float (&q)[V], float n, float2* red, int pitch)
 {
 #pragma unroll
     for (int e = 0; e < V / SUB; e++)
@@ -217,12 +218,12 @@ __device__ __forceinline__ void merge_channels(const float (&m)[V], const float 
             const float d = m[e * SUB + j] - mean;
             m2 += q[e * SUB + j] + n * d * d;
         }
-        red[e] = make_float2(mean, m2);
+        red[e * pitch] = make_float2(mean, m2);
     }
 }
 template <int V>
 __device__ __forceinline__ void leave_sums(const float2 (&neg)[kPairs<V>], const float2 (&s1)[kPairs<V>],
-                                           const float2 (&s2)[kPairs<V>], int n, int sub, float2* red)
+                                           const float2 (&s2)[kPairs<V>], int n, int sub, float2* red, int pitch)
 {
     const float fn = (float)n, inv = __fdividef(1.f, fn);
     float m[V], q[V];
@@ -235,13 +236,13 @@ __device__ __forceinline__ void leave_sums(const float2 (&neg)[kPairs<V>], const
         q[j] = not_negative(b - a * mean);
     }
     if (V == 8 && sub == 8)
-        merge_channels<V, V>(m, q, fn, red);
+        merge_channels<V, V>(m, q, fn, red, pitch);
     else if (V >= 4 && sub == 4)
-        merge_channels<V, V >= 4 ? 4 : 1>(m, q, fn, red);
+        merge_channels<V, V >= 4 ? 4 : 1>(m, q, fn, red, pitch);
     else if (V >= 4 && sub == 2)
-        merge_channels<V, V >= 4 ? 2 : 1>(m, q, fn, red);
+        merge_channels<V, V >= 4 ? 2 : 1>(m, q, fn, red, pitch);
     else
-        merge_channels<V, 1>(m, q, fn, red);
+        merge_channels<V, 1>(m, q, fn, red, pitch);
 }
 
 // Thread t of a CTA owns vector column t % cols and rows t / cols, + slots, ...
@@ -260,6 +261,10 @@ struct Lanes
     __device__ int rows_of(int s) const { return rounds + (s < more ? 1 : 0); }
     __device__ int mine() const { return slot < slots ? rows_of(slot) : 0; }
     __device__ int live_slots() const { return rounds > 0 ? slots : more; }
+    // Entries of the reduction lie unit after unit (a unit: `sub` channels), a
+    // unit's slots side by side; the odd pitch keeps both ways of walking them
+    // off one bank.
+    __device__ int pitch() const { return slots | 1; }
 };
 
 template <int V>
@@ -357,9 +362,15 @@ __device__ __forceinline__ void st_cluster_v4(uint32_t addr, float4 v)
 // ---------------------------------------------------------------- slab kernel
 constexpr int kHeld = 8; // rows of its vector column per thread, in registers
 
-size_t slab_smem(int cluster, int groups, int per_thread)
+// Bytes of the reduction: units x pitch.
+size_t red_bytes(int cols, int per_thread)
 {
-    return (size_t)(cluster + 1) * groups * 16 + (size_t)groups * 8 + (size_t)kThreads * per_thread * 8;
+    return ((size_t)cols * per_thread * ((kThreads / cols) | 1) * 8 + 15) / 16 * 16;
+}
+
+size_t slab_smem(int cluster, int groups, int cols, int per_thread)
+{
+    return (size_t)(cluster + 1) * groups * 16 + (size_t)groups * 8 + red_bytes(cols, per_thread);
 }
 
 template <typename TI, typename TO, int V>
@@ -402,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_norm_slab_kernel(const Grou
                 unpack<TI, V>(raw[k], f);
                 s.add(f);
             }
-        leave_sums<V>(s.neg, s.s1, s.s2, mine, a.sub, red + threadIdx.x * per_thread);
+        leave_sums<V>(s.neg, s.s1, s.s2, mine, a.sub, red + t.col * per_thread * t.pitch() + t.slot, t.pitch());
     }
     // every CTA of the cluster runs before any writes into its shared memory
     if (P > 1)
@@ -414,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_norm_slab_kernel(const Grou
     join_groups(
         0, G, t.live_slots(), units,
         [&](int g, int sl, int u) {
-            const float2 v = red[sl * t.cols * per_thread + g * units + u];
+            const float2 v = red[(g * units + u) * t.pitch() + sl];
             return make_float3((float)(t.rows_of(sl) * a.sub), v.x, v.y);
         },
         [&](int g, float3 j) {
@@ -526,37 +537,34 @@ struct RowStream
     {
         if constexpr (V > 1)
         {
-            int left = n;
-            while (left > 0)
+            // not unrolled over the ring: with four activations' bodies in it the
+            // loop would outgrow the instruction cache
+            int slot = 0;
+            for (int left = n; left > 0; left -= kStep)
             {
-#pragma unroll
-                for (int d = 0; d < kDepth; d++)
+                asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+                Raw<TI, V> r;
+                const uint8_t* at = mine + slot * (kStep * ROW);
+                if (left >= kStep)
                 {
-                    if (left <= 0) break;
-                    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
-                    Raw<TI, V> r;
-                    const uint8_t* at = mine + d * (kStep * ROW);
-                    if (left >= kStep)
-                    {
 #pragma unroll
-                        for (int u = 0; u < kStep; u++)
-                        {
-                            r.q = *reinterpret_cast<const decltype(r.q)*>(at + u * ROW);
-                            f(r);
-                        }
-                    }
-                    else
+                    for (int u = 0; u < kStep; u++)
                     {
-#pragma unroll 1
-                        for (int u = 0; u < left; u++)
-                        {
-                            r.q = *reinterpret_cast<const decltype(r.q)*>(at + u * ROW);
-                            f(r);
-                        }
+                        r.q = *reinterpret_cast<const decltype(r.q)*>(at + u * ROW);
+                        f(r);
                     }
-                    left -= kStep;
-                    fetch((d + kDepth - 1) % kDepth); // into the slot that the step before has read
                 }
+                else
+                {
+#pragma unroll 1
+                    for (int u = 0; u < left; u++)
+                    {
+                        r.q = *reinterpret_cast<const decltype(r.q)*>(at + u * ROW);
+                        f(r);
+                    }
+                }
+                fetch(slot == 0 ? kDepth - 1 : slot - 1); // into the slot that the step before has read
+                slot = slot == kDepth - 1 ? 0 : slot + 1;
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
@@ -599,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) group_norm_sums_kernel(cons
     float4* own = reinterpret_cast<float4*>(smem); // [G]
     float2* red = reinterpret_cast<float2*>(own + G);
     cudaTriggerProgrammaticLaunchCompletion(); // the apply kernel waits for the results itself
-    uint8_t* ring = reinterpret_cast<uint8_t*>(red + kThreads * (V / a.sub));
+    uint8_t* ring = reinterpret_cast<uint8_t*>(red) + a.red_bytes;
     const int per_thread = V / a.sub;
     const Part p(a);
     const int vpr = a.slice / V;
@@ -625,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) group_norm_sums_kernel(cons
                 unpack<TI, V>(raw, f);
                 s.add(f);
             });
-            leave_sums<V>(s.neg, s.s1, s.s2, mine, a.sub, red + threadIdx.x * per_thread);
+            leave_sums<V>(s.neg, s.s1, s.s2, mine, a.sub, red + t.col * per_thread * t.pitch() + t.slot, t.pitch());
         }
         __syncthreads();
         const int ch0 = cb * V, ch1 = min(vpr, cb + t.cols) * V;
@@ -635,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) group_norm_sums_kernel(cons
             join_groups(
                 0, G, t.live_slots(), units,
                 [&](int g, int sl, int u) {
-                    const float2 v = red[sl * t.cols * per_thread + g * units + u];
+                    const float2 v = red[(g * units + u) * t.pitch() + sl];
                     return make_float3((float)(t.rows_of(sl) * a.sub), v.x, v.y);
                 },
                 [&](int g, float3 j) { own[g] = make_float4(j.x, j.y, j.z, 0.f); });
@@ -647,12 +655,12 @@ __global__ void __launch_bounds__(kThreads, kBlocks) group_norm_sums_kernel(cons
             for (int g = ch0 / a.width + warp; g * a.width < ch1; g += kWarps)
             {
                 const int lo = max(g * a.width, ch0), units = (min((g + 1) * a.width, ch1) - lo) / a.sub;
-                const float2* entry = red + (lo - ch0) / a.sub;
+                const float2* entry = red + (lo - ch0) / a.sub * t.pitch();
                 float3 j = make_float3(0.f, 0.f, 0.f);
                 for (int sl = 0; sl < t.live_slots(); sl++)
                     for (int u = lane; u < units; u += 32)
                     {
-                        const float2 v = entry[sl * t.cols * per_thread + u];
+                        const float2 v = entry[u * t.pitch() + sl];
                         j = join2(j, make_float3((float)(t.rows_of(sl) * a.sub), v.x, v.y));
                     }
 #pragma unroll
@@ -756,6 +764,9 @@ struct Cut
 //   14,400 x 512 bf16: 45.5 us at 444 parts, 49.9 at 296, 52.8 at 888).
 constexpr int kSlabCtas = 2 * 148;
 constexpr int kPartCtas = kBlocks * 148;
+// Values a CTA at least: with fewer its set-up costs more than it saves (6 x
+// 4,282 x 128 17.7 us at 8,192, 15.0 at 16,384; 1 x 53,217 x 33 12.3 and 14.7).
+constexpr int kPartMin = 16384;
 
 Cut cut(int64_t instances, int64_t rows, int C, int width, int V)
 {
@@ -775,7 +786,7 @@ Cut cut(int64_t instances, int64_t rows, int C, int width, int V)
         const int u8 = width / gcd(width, 8) * 8, u4 = width / gcd(width, 4) * 4;
         c.slice = widest_slice(C, C % u8 == 0 ? u8 : (C % u4 == 0 ? u4 : width), 128);
         const int64_t runs = instances * (C / c.slice);
-        c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kPartCtas / runs, (rows + 31) / 32));
+        c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kPartCtas / runs, rows * c.slice / kPartMin));
     }
     return c;
 }
@@ -832,6 +843,7 @@ int launch(Context& ctx, GroupNormArgs a, int instances, int C, void* workspace)
     a.parts = c.parts;
     const int cols = std::min(kThreads, a.slice / V);
     a.slots = kThreads / cols;
+    a.red_bytes = (int)red_bytes(cols, V / a.sub);
     a.by_cols = (uint32_t)(((1ull << 32) + cols - 1) / cols);
     a.part_rows = a.rows / c.parts;
     a.longer = a.rows - a.part_rows * c.parts;
@@ -842,12 +854,12 @@ int launch(Context& ctx, GroupNormArgs a, int instances, int C, void* workspace)
     {
         static std::atomic<uint64_t> seen{0};
         return launch_kernel(ctx, group_norm_slab_kernel<TI, TO, V>, seen, grid, a.parts,
-                             slab_smem(a.parts, a.groups, V / a.sub), false, a);
+                             slab_smem(a.parts, a.groups, cols, V / a.sub), false, a);
     }
     a.partial = static_cast<float2*>(workspace);
     static std::atomic<uint64_t> seen_sums{0}, seen_apply{0};
     const int r = launch_kernel(ctx, group_norm_sums_kernel<TI, V>, seen_sums, grid, 1,
-                                (size_t)a.groups * 16 + (size_t)kThreads * (V / a.sub) * 8 + kRingBytes<TI, V>, false, a);
+                                (size_t)a.groups * 16 + red_bytes(cols, V / a.sub) + kRingBytes<TI, V>, false, a);
     if (r != S2_OK) return r;
     return launch_kernel(ctx, group_norm_apply_kernel<TI, TO, V>, seen_apply, grid, 1, ((size_t)a.groups * 8 + 15) / 16 * 16 + kRingBytes<TI, V>, true, a);
 }
