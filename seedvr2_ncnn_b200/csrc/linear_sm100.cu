@@ -24,13 +24,20 @@ constexpr int kMaxGroups = 1024;
 constexpr size_t kSmemLimit = 232448;
 
 // The tensor core adds into its fp32 accumulator without rounding to nearest:
-// over K = 10,240 an fp32 result is then off by 1.2e-5 of itself (5.2e-6
-// measured under a gate and a residual).  Where the result is fp32 and K is
-// longer than kLongK blocks, sums of kChunk blocks are therefore added up in
-// fp32 registers (or shared memory) instead, each while the tensor core works
-// on the next one.  A bf16 result rounds at 2^-9 and keeps one sum.
-constexpr int kChunk = 24;
-constexpr int kLongK = 24;
+// an fp32 result is off by 6e-8 of itself for each K block in one sum (1.2e-5
+// over K = 10,240).  Where the result is fp32, sums of at most kChunk blocks
+// (9e-7) are therefore added up in fp32 registers (or shared memory), each while
+// the tensor core works on the next one: 21,658 x 2,560 x 10,240 takes 898 us so
+// (869 at 24 blocks, 916 at 12) and 835 in one sum.  A bf16 result rounds at
+// 2^-9 and keeps one sum.
+constexpr int kChunk = 16;
+
+// Blocks of one sum: equal ones.
+constexpr int chunk_blocks(int num_kb, bool out_f32)
+{
+    const int chunks = out_f32 ? (num_kb + kChunk - 1) / kChunk : 1;
+    return (num_kb + chunks - 1) / chunks;
+}
 
 struct LinearArgs
 {
@@ -1271,7 +1278,7 @@ int launch_tiles(Context& ctx, const Operands& o, const BoxMaps& m, LinearArgs a
     a.nblk = (a.N + BN - 1) / BN;
     a.stages = TL::stages(a.groups);
     a.group_m = a.K >= 8192 ? 1 : (a.N <= 4096 ? 8 : 16);
-    a.chunk_kb = SUM ? kChunk : a.num_kb;
+    a.chunk_kb = chunk_blocks(a.num_kb, SUM);
     const int64_t units = ((int64_t)a.rows / (CTAS * BM) + a.groups) * a.nblk; // at most
     if (units > 0x7fffffff) return S2_ERR_INVALID;
     const size_t smem = TL::fixed_bytes(a.groups) + (size_t)a.stages * TL::STAGE_BYTES;
@@ -1355,7 +1362,7 @@ int launch_rows(Context& ctx, const Operands& o, LinearArgs a)
     if (a.groups > 1 && mean_rows > 8) row_tiles = std::max(row_tiles, 4);
     if ((int64_t)a.groups * a.nblk * s > 0x7fffffff) return S2_ERR_INVALID;
     a.cluster = s;
-    a.chunk_kb = a.out_f32 && a.num_kb > kLongK ? kChunk : a.num_kb;
+    a.chunk_kb = chunk_blocks((a.num_kb + s - 1) / s, a.out_f32);
     const int esz = a.out_f32 ? 4 : 2;
     a.vec_out = reinterpret_cast<uintptr_t>(a.out) % (4 * esz) == 0 && a.out_ld % 4 == 0;
     a.vec_res = reinterpret_cast<uintptr_t>(a.residual) % (4 * esz) == 0 && a.residual_ld % 4 == 0;
@@ -1452,7 +1459,7 @@ int run_linear(s2_context* ctx, int rows, int groups, const int* offsets, int N,
     // for sums from a fifth (21,658 x 2,560 x 2,560 with an fp32 residual 265
     // against 281 us; x 10,240: 869 against 847).
     const double moved = 128.0 * 256 * osz, fed = (double)a.num_kb * 32768;
-    if (a.out_f32 && a.num_kb > kLongK)
+    if (a.out_f32 && a.num_kb > kChunk)
     {
         if (!pair) return launch_tiles<1, 128, 2, 8, true>(c, o, m, a);
         return moved >= 0.2 * fed ? launch_tiles<2, 256, 3, 8, true>(c, o, m, a)

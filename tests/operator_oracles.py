@@ -40,7 +40,8 @@ def activated(x, dx, act, fast=False):
 
 def linear(a, w, bias, act, gate, residual, dtype):
     """(out, bound).  Products of bf16 are exact in fp32; the tensor core adds K of them in steps of 16 into an fp32
-    accumulator, each step off by at most a whole step (2 U) of the partial sum, which sum |a| |w| bounds."""
+    accumulator, each step off by at most a whole step (2 U) of the partial sum, which sum |a| |w| bounds; splitting
+    the sum only shortens that."""
     a, w = a.double(), w.double()
     x = a @ w.t()
     s = a.abs() @ w.abs().t()

@@ -39,7 +39,8 @@ def _case(seed, rows, n, k, *, groups=None, bias=True, gate=False, residual=Fals
 
 SIZES = [(1, 8, 8), (1, 1, 1), (1, 2560, 2560), (3, 130, 72), (16, 128, 64), (17, 1001, 131), (58, 640, 2560),
          (64, 129, 65), (65, 129, 65), (128, 128, 128), (200, 96, 40), (300, 515, 1000), (1000, 1536, 520),
-         (2049, 2560, 128), (4001, 1304, 264), (6000, 1023, 72), (20000, 256, 192)]
+         (2049, 2560, 128), (4001, 1304, 264), (6000, 1023, 72), (20000, 256, 192),
+         (40, 200, 5000), (150, 1300, 2050), (2049, 2560, 1096), (2500, 2055, 1030)]
 
 
 @pytest.mark.parametrize("size", SIZES, ids=str)
@@ -133,6 +134,56 @@ def test_grouped_linear(s2lib, gpu_ctx, layout, form):
     s2lib.grouped_linear(gpu_ctx, a, w, off, b, act=oracles.ACTS.index(act), gate=gt, residual=res, out=got)
     assert gpu_ctx.status() == 0
     oracles.check(got, *oracles.grouped_linear(a, w, offsets, b, act, gt, res, DT[out], before), f"{layout} {form}")
+
+
+@pytest.mark.parametrize("layout", [([0, 58, 700], 700), ([3, 3, 20, 20, 21, 37], 50), ([0, 130, 130, 131, 387, 900, 901], 930),
+                                    ([0, 6000, 6058], 6058), ([0] + [300 * i + 7 for i in range(1, 17)], 5000)],
+                         ids=lambda v: f"{len(v[0]) - 1}x{v[1]}")
+@pytest.mark.parametrize("n", [640, 643])
+def test_grouped_linear_long_sums(s2lib, gpu_ctx, layout, n):
+    """fp32 results over more K than one accumulator sums (17 blocks of 64: two sums)."""
+    offsets, rows = layout
+    a, w, b, gt, res = _case(rows, rows, n, 1030, groups=len(offsets) - 1, gate=True, residual=True, out="f32")
+    got = torch.full((rows, n), 2.0, device="cuda")
+    before = got.clone()
+    s2lib.grouped_linear(gpu_ctx, a, w, torch.tensor(offsets, dtype=torch.int32, device="cuda"), b,
+                         act=s2lib.S2_ACT_GELU_ERF, gate=gt, residual=res, out=got)
+    assert gpu_ctx.status() == 0
+    oracles.check(got, *oracles.grouped_linear(a, w, offsets, b, "gelu_erf", gt, res, torch.float32, before))
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300, 2500])
+def test_fp32_results_keep_their_precision(s2lib, gpu_ctx, rows):
+    """K = 10,240 without a residual: the 2-norm of the error stays at 2e-6 of the result's (sums of 16 blocks of 64
+    lose 16 steps of 4 products' worth, some 6e-8 a block, whatever K is; one sum of 160 blocks lost 1.2e-5)."""
+    a, w, _, _, _ = _case(9, rows, 384, 10240, bias=False, out="f32")
+    got = s2lib.linear(gpu_ctx, a, w, out_dtype=s2lib.S2_DTYPE_F32).double()
+    want = a.double() @ w.double().t()
+    assert float((got - want).norm() / want.norm()) < 2e-6
+
+
+def test_linear_captured(s2lib, gpu_ctx):
+    """Each kernel of the product in one graph, replayed on other values."""
+    cases = [_case(30 + i, *size, residual=True, out="f32") for i, size in enumerate(
+        ((3, 260, 520), (200, 640, 1400), (5000, 640, 1400), (5000, 643, 200)))]
+    outs = [torch.zeros_like(c[4]) for c in cases]
+    run = lambda: [s2lib.linear(gpu_ctx, c[0], c[1], c[2], residual=c[4], out=o) for c, o in zip(cases, outs)]  # noqa: E731
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    home = gpu_ctx.stream
+    with torch.cuda.graph(graph):
+        gpu_ctx.set_stream(torch.cuda.current_stream())
+        run()
+    gpu_ctx.set_stream(home)
+    for c in cases:
+        c[4].mul_(2)
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [o.clone() for o in outs]
+    run()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, outs))
+    del graph
 
 
 @pytest.mark.parametrize("rows", [30, 4000])
