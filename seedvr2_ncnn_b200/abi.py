@@ -495,18 +495,35 @@ def _vector(t, shape, device: int, what: str):
     return t.data_ptr()
 
 
-def _new(ctx, shape, code):
+def _new(ctx, shape, dtype):
+    """Memory for a call on the context's stream: from that stream's own pool, so that it waits for whatever used it
+    there before, and kept for the work of torch's current stream, where the caller takes it."""
     import torch
 
-    return torch.empty(shape, device=torch.device("cuda", ctx.device),
-                       dtype=torch.float32 if code == S2_DTYPE_F32 else torch.bfloat16)
+    device = torch.device("cuda", ctx.device)
+    current = torch.cuda.current_stream(device)
+    if current == ctx.stream:
+        return torch.empty(shape, device=device, dtype=dtype)
+    with torch.cuda.stream(ctx.stream):
+        t = torch.empty(shape, device=device, dtype=dtype)
+    t.record_stream(current)
+    return t
+
+
+def _new_out(ctx, shape, code):
+    import torch
+
+    return _new(ctx, shape, torch.float32 if code == S2_DTYPE_F32 else torch.bfloat16)
 
 
 def _operand_stride(t, device: int, what: str) -> int:
-    """Row stride of a bf16 operand; a single row, which has none of its own, gets its length rounded up to 8."""
+    """Row stride of a bf16 operand; one row or none, which have none of their own, get the length rounded up to 8."""
     _require(_dtype_code(t, what) == S2_DTYPE_BF16 and t.get_device() == device, what)
     k = t.shape[-1]
-    return (k + 7) // 8 * 8 if t.numel() == k else _row_stride(t, what)
+    if t.numel() > k:
+        return _row_stride(t, what)
+    _require(t.numel() < 2 or t.stride(-1) == 1, what)
+    return (k + 7) // 8 * 8
 
 
 def _linear(ctx, what, a, weight, offsets, bias, act, gate, residual, out_dtype, out):
@@ -516,9 +533,11 @@ def _linear(ctx, what, a, weight, offsets, bias, act, gate, residual, out_dtype,
     _require(len(a_shape) == 2 and len(w_shape) == (3 if grouped else 2) and w_shape[-1] == a_shape[1], what)
     rows, K = a_shape
     N = w_shape[-2]
+    # a C int drops what it does not hold
+    _require(rows < 2**31 and N < 2**31 and K < 2**31, what)
     lda, ldw = _operand_stride(a, dev, what), _operand_stride(weight, dev, what)
     if out is None:
-        out = _new(ctx, (rows, N), out_dtype)
+        out = _new_out(ctx, (rows, N), out_dtype)
     code = _dtype_code(out, what)
     _require(out.shape == (rows, N) and out.get_device() == dev, what)
     vec = w_shape[:-1]  # (N,), or (groups, N)
@@ -568,9 +587,10 @@ def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=
     rows = 1
     for n in shape[1:-1]:
         rows *= n
+    _require(instances < 2**31 and channels < 2**31 and 0 < groups <= channels, what)
     code = _dtype_code(x, what)
     if out is None:
-        out = _new(ctx, shape, code if out_dtype is None else out_dtype)
+        out = _new_out(ctx, shape, code if out_dtype is None else out_dtype)
     out_code = _dtype_code(out, what)
     _require(out.shape == shape and out.get_device() == dev, what)
     L = lib()
@@ -579,8 +599,7 @@ def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=
     if need:
         import torch
 
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        ws.record_stream(ctx.stream)  # freed here, used there
+        ws = _new(ctx, need, torch.uint8)
     vec = (channels,)
     check(L.s2_group_norm(ctx.handle, instances, rows, channels, groups, code, x.data_ptr(), _row_stride(x, what),
                           _vector(gamma, vec, dev, what), _vector(beta, vec, dev, what), eps, act, out_code,

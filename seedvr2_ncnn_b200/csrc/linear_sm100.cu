@@ -56,7 +56,6 @@ struct LinearArgs
     int stages;
     int group_m; // M blocks per raster group
     int chunk_kb; // K blocks summed by the tensor core before the sum is taken over (see kChunk)
-    int cluster;  // linear_rows_kernel: K parts
     int vec_out, vec_res; // linear_rows_kernel: four outputs / residuals at once
     int* status;
 };
@@ -1361,7 +1360,6 @@ int launch_rows(Context& ctx, const Operands& o, LinearArgs a)
         if (p <= a.num_kb && units * row_tiles * p <= room) s = p;
     if (a.groups > 1 && mean_rows > 8) row_tiles = std::max(row_tiles, 4);
     if ((int64_t)a.groups * a.nblk * s > 0x7fffffff) return S2_ERR_INVALID;
-    a.cluster = s;
     a.chunk_kb = chunk_blocks((a.num_kb + s - 1) / s, a.out_f32);
     const int esz = a.out_f32 ? 4 : 2;
     a.vec_out = reinterpret_cast<uintptr_t>(a.out) % (4 * esz) == 0 && a.out_ld % 4 == 0;

@@ -254,6 +254,29 @@ def test_two_contexts_on_two_streams(s2lib, gpu_ctx):
         ctxs[i].close()
 
 
+def test_memory_of_a_call_on_another_stream(s2lib, gpu_ctx):
+    """The memory that a call on its own stream gets is not one that torch's current stream has yet to write to."""
+    a, w, b, _, _ = _case(7, 900, 640, 520)
+    x = torch.randn(2, 20000, 128, device="cuda").bfloat16()
+    want, want_norm = s2lib.linear(gpu_ctx, a, w, b), s2lib.group_norm(gpu_ctx, x, 32)
+    need = s2lib.lib().s2_group_norm_workspace(2, 20000, 128, 32)
+    assert need > 0
+    stream = torch.cuda.Stream()
+    ctx = s2lib.Context(0, stream)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        torch.cuda._sleep(20_000_000)
+        for like in (want, want_norm):
+            torch.full_like(like, 7)
+        torch.full((need,), 255, dtype=torch.uint8, device="cuda")  # all three freed with their writes to come
+        y, y_norm = s2lib.linear(ctx, a, w, b), s2lib.group_norm(ctx, x, 32)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(y_norm, want_norm)
+        del y, y_norm
+    assert ctx.status() == 0
+    ctx.close()
+
+
 def test_wrapper_refuses(s2lib, gpu_ctx):
     a, w, b, _, _ = _case(1, 8, 16, 16)
     bad = [lambda: s2lib.linear(gpu_ctx, a.float(), w), lambda: s2lib.linear(gpu_ctx, a, w.float()),

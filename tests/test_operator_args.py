@@ -113,6 +113,59 @@ def test_row_strides(s2lib):
             stride(bad)
 
 
+def test_operand_strides(s2lib):
+    stride = lambda t: s2lib._operand_stride(t, -1, "t")  # noqa: E731
+    rows = lambda *shape: torch.empty(shape, dtype=torch.bfloat16)  # noqa: E731
+    assert stride(rows(4, 16)) == 16 and stride(rows(4, 24)[:, :13]) == 24
+    assert stride(rows(1, 13)) == 16 and stride(rows(4, 24)[2:3, :13]) == 16, "a row of its own has no stride"
+    assert stride(rows(0, 13)) == 16 and stride(rows(4, 24)[:0, :13]) == 16, "nor have no rows"
+    assert stride(rows(3, 1)[:1]) == 8
+    for bad in (rows(13, 4).t()[:1], rows(1, 26)[:, ::2], rows(4, 26)[:, ::2]):
+        with pytest.raises(s2lib.S2Error):
+            stride(bad)
+
+
+class _Sized:
+    """The size of a tensor and an address that is never followed."""
+
+    def __init__(self, shape, dtype, address):
+        self.meta, self.address = torch.empty(shape, dtype=dtype, device="meta"), address
+        self.shape, self.dtype = self.meta.shape, dtype
+
+    def __getattr__(self, name):
+        return getattr(self.meta, name)
+
+    def get_device(self):
+        return -1
+
+    def data_ptr(self):
+        return self.address
+
+
+def test_wrappers_refuse_what_a_c_int_does_not_hold(s2lib, ctx):
+    class Ctx:
+        handle, device = ctx, -1
+
+    bf16 = lambda shape, at: _Sized(shape, torch.bfloat16, at)  # noqa: E731
+
+    def linear(m, n, k):
+        s2lib.linear(Ctx, bf16((m, k), BASE), bf16((n, k), BASE), out=bf16((m, n), OUT))
+
+    def norm(instances, groups, channels=32):
+        x = bf16((instances, 5, channels), BASE)
+        s2lib.group_norm(Ctx, x, groups, out=bf16(x.shape, OUT))
+
+    for call, good, bad in ((linear, (5, 16, 16), [(2**32 + 5, 16, 16), (5, 2**32 + 16, 16), (5, 16, 2**32 + 16)]),
+                            (norm, (2, 4), [(2**32 + 2, 4), (2, 2**32 + 4), (2, 4, 2**32 + 32), (2, 0), (2, -4)])):
+        with pytest.raises(s2lib.S2Error) as e:
+            call(*good)
+        assert e.value.code == s2lib.S2_ERR_CUDA
+        for args in bad:
+            with pytest.raises(s2lib.S2Error) as e:
+                call(*args)
+            assert e.value.code == s2lib.S2_ERR_INVALID, args
+
+
 def test_oracles_agree_with_torch():
     """The 64-bit restatements against torch's own layers."""
     g = torch.Generator().manual_seed(1)
