@@ -449,26 +449,33 @@ def shared_linear(ctx: Context, a0, weight, bias=None, *, a1=None, epilogue=S2_E
     return out0, out1
 
 
-def _require(ok: bool, what: str) -> None:
-    if not ok:
-        raise S2Error(S2_ERR_INVALID, what)
+# The checks below stand in the path of calls that take the device a few
+# microseconds, so they are written out rather than factored: each Python call
+# costs some 50 ns, each attribute of a tensor as much.
+def _refuse(what: str):
+    raise S2Error(S2_ERR_INVALID, what)
 
 
 def _row_stride(t, what: str) -> int:
     """Row stride (elements) of a tensor whose last dimension is dense and whose leading ones are one run of rows."""
     shape = t.shape
-    _require(len(shape) >= 2, what)
-    if t.is_contiguous() or t.numel() == 0:
+    if t.is_contiguous() and len(shape) >= 2:
+        return shape[-1]
+    if len(shape) < 2:
+        _refuse(what)
+    if t.numel() == 0:
         return shape[-1]
     strides = t.stride()
-    _require(shape[-1] == 1 or strides[-1] == 1, what)
+    if shape[-1] != 1 and strides[-1] != 1:
+        _refuse(what)
     ld = None
     run = 1  # rows below the dimension
     for d in range(len(shape) - 2, -1, -1):
         if shape[d] != 1:
             if ld is None:
                 ld = strides[d]
-            _require(strides[d] == ld * run, what)
+            if strides[d] != ld * run:
+                _refuse(what)
         run *= shape[d]
     return shape[-1] if ld is None else ld
 
@@ -476,22 +483,20 @@ def _row_stride(t, what: str) -> int:
 _codes = {}
 
 
-def _dtype_code(t, what: str) -> int:
+def _dtype_codes():
+    """S2_DTYPE_* of the torch types there is one for."""
     if not _codes:
         import torch
 
         _codes.update({torch.float32: S2_DTYPE_F32, torch.bfloat16: S2_DTYPE_BF16})
-    code = _codes.get(t.dtype)
-    _require(code is not None, what)
-    return code
+    return _codes
 
 
 def _vector(t, shape, device: int, what: str):
-    """Address of an optional dense fp32 tensor of this shape."""
-    if t is None:
-        return None
-    _require(_dtype_code(t, what) == S2_DTYPE_F32 and t.shape == shape and t.get_device() == device
-             and t.is_contiguous(), what)
+    """Address of a dense fp32 tensor of this shape."""
+    if (_codes.get(t.dtype) != S2_DTYPE_F32 or t.shape != shape or t.get_device() != device
+            or not t.is_contiguous()):
+        _refuse(what)
     return t.data_ptr()
 
 
@@ -516,46 +521,56 @@ def _new_out(ctx, shape, code):
     return _new(ctx, shape, torch.float32 if code == S2_DTYPE_F32 else torch.bfloat16)
 
 
-def _operand_stride(t, device: int, what: str) -> int:
+def _operand_stride(t, shape, device: int, what: str) -> int:
     """Row stride of a bf16 operand; one row or none, which have none of their own, get the length rounded up to 8."""
-    _require(_dtype_code(t, what) == S2_DTYPE_BF16 and t.get_device() == device, what)
-    k = t.shape[-1]
-    if t.numel() > k:
-        return _row_stride(t, what)
-    _require(t.numel() < 2 or t.stride(-1) == 1, what)
+    if (_codes or _dtype_codes()).get(t.dtype) != S2_DTYPE_BF16 or t.get_device() != device:
+        _refuse(what)
+    k = shape[-1]
+    n = t.numel()
+    if n > k:
+        return k if t.is_contiguous() else _row_stride(t, what)
+    if n > 1 and t.stride(-1) != 1:
+        _refuse(what)
     return (k + 7) // 8 * 8
 
 
 def _linear(ctx, what, a, weight, offsets, bias, act, gate, residual, out_dtype, out):
     dev = ctx.device
+    codes = _codes or _dtype_codes()
     a_shape, w_shape = a.shape, weight.shape
-    grouped = offsets is not None
-    _require(len(a_shape) == 2 and len(w_shape) == (3 if grouped else 2) and w_shape[-1] == a_shape[1], what)
+    if len(a_shape) != 2 or len(w_shape) != (2 if offsets is None else 3) or w_shape[-1] != a_shape[1]:
+        _refuse(what)
     rows, K = a_shape
     N = w_shape[-2]
-    # a C int drops what it does not hold
-    _require(rows < 2**31 and N < 2**31 and K < 2**31, what)
-    lda, ldw = _operand_stride(a, dev, what), _operand_stride(weight, dev, what)
+    if rows >= 2**31 or N >= 2**31 or K >= 2**31:  # a C int drops what it does not hold
+        _refuse(what)
+    lda, ldw = _operand_stride(a, a_shape, dev, what), _operand_stride(weight, w_shape, dev, what)
     if out is None:
         out = _new_out(ctx, (rows, N), out_dtype)
-    code = _dtype_code(out, what)
-    _require(out.shape == (rows, N) and out.get_device() == dev, what)
-    vec = w_shape[:-1]  # (N,), or (groups, N)
-    e = LinearEpilogue(act, _vector(bias, vec, dev, what), _vector(gate, vec, dev, what), None, 0)
+    code = codes.get(out.dtype)
+    if code is None or out.shape != (rows, N) or out.get_device() != dev:
+        _refuse(what)
+    e = LinearEpilogue(act)
+    if bias is not None:
+        e.bias = _vector(bias, w_shape[:-1], dev, what)
+    if gate is not None:
+        e.gate = _vector(gate, w_shape[:-1], dev, what)
     if residual is not None:
-        _require(residual.dtype == out.dtype and residual.shape == out.shape and residual.get_device() == dev, what)
+        if residual.dtype != out.dtype or residual.shape != out.shape or residual.get_device() != dev:
+            _refuse(what)
         e.residual = residual.data_ptr()
         e.residual_ld = _row_stride(residual, what)
     ldo = N if out.is_contiguous() else _row_stride(out, what)
-    if grouped:
-        groups = w_shape[0]
-        _require(offsets.element_size() == 4 and not offsets.is_floating_point() and offsets.shape == (groups + 1,)
-                 and offsets.is_contiguous() and offsets.get_device() == dev, what)
-        r = lib().s2_grouped_linear(ctx.handle, rows, groups, offsets.data_ptr(), N, K, a.data_ptr(), lda,
-                                    weight.data_ptr(), ldw, C.byref(e), code, out.data_ptr(), ldo)
-    else:
+    if offsets is None:
         r = lib().s2_linear(ctx.handle, rows, N, K, a.data_ptr(), lda, weight.data_ptr(), ldw, C.byref(e), code,
                             out.data_ptr(), ldo)
+    else:
+        groups = w_shape[0]
+        if (offsets.element_size() != 4 or offsets.is_floating_point() or offsets.shape != (groups + 1,)
+                or not offsets.is_contiguous() or offsets.get_device() != dev):
+            _refuse(what)
+        r = lib().s2_grouped_linear(ctx.handle, rows, groups, offsets.data_ptr(), N, K, a.data_ptr(), lda,
+                                    weight.data_ptr(), ldw, C.byref(e), code, out.data_ptr(), ldo)
     if r:
         check(r, what)
     return out
@@ -572,7 +587,8 @@ def grouped_linear(ctx: Context, a, weight, offsets, bias=None, *, act=S2_ACT_NO
                    out_dtype=S2_DTYPE_BF16, out=None):
     """linear() with weight [G, N, K], bias / gate [G, N] of group g for rows offsets[g] <= r < offsets[g + 1]
     (int32 CUDA tensor [G + 1]); other rows of out are left as they were (unset when out is made here)."""
-    _require(offsets is not None, "s2_grouped_linear")
+    if offsets is None:
+        _refuse("s2_grouped_linear")
     return _linear(ctx, "s2_grouped_linear", a, weight, offsets, bias, act, gate, residual, out_dtype, out)
 
 
@@ -581,18 +597,26 @@ def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=
     channel group over the dimensions between; gamma / beta fp32 [channels].  out: x's shape (x itself in place)."""
     what = "s2_group_norm"
     dev = ctx.device
+    codes = _codes or _dtype_codes()
     shape = x.shape
-    _require(len(shape) >= 2 and x.get_device() == dev, what)
+    code = codes.get(x.dtype)
+    if len(shape) < 2 or code is None or x.get_device() != dev:
+        _refuse(what)
     instances, channels = shape[0], shape[-1]
     rows = 1
     for n in shape[1:-1]:
         rows *= n
-    _require(instances < 2**31 and channels < 2**31 and 0 < groups <= channels, what)
-    code = _dtype_code(x, what)
+    if instances >= 2**31 or channels >= 2**31 or not 0 < groups <= channels:  # a C int drops what it does not hold
+        _refuse(what)
     if out is None:
         out = _new_out(ctx, shape, code if out_dtype is None else out_dtype)
-    out_code = _dtype_code(out, what)
-    _require(out.shape == shape and out.get_device() == dev, what)
+    out_code = codes.get(out.dtype)
+    if out_code is None or out.shape != shape or out.get_device() != dev:
+        _refuse(what)
+    if gamma is not None:
+        gamma = _vector(gamma, shape[-1:], dev, what)
+    if beta is not None:
+        beta = _vector(beta, shape[-1:], dev, what)
     L = lib()
     need = L.s2_group_norm_workspace(instances, rows, channels, groups)
     ws = None
@@ -600,10 +624,11 @@ def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=
         import torch
 
         ws = _new(ctx, need, torch.uint8)
-    vec = (channels,)
-    check(L.s2_group_norm(ctx.handle, instances, rows, channels, groups, code, x.data_ptr(), _row_stride(x, what),
-                          _vector(gamma, vec, dev, what), _vector(beta, vec, dev, what), eps, act, out_code,
-                          out.data_ptr(), _row_stride(out, what), ptr(ws), need), what)
+    r = L.s2_group_norm(ctx.handle, instances, rows, channels, groups, code, x.data_ptr(), _row_stride(x, what), gamma,
+                        beta, eps, act, out_code, out.data_ptr(), _row_stride(out, what),
+                        ws.data_ptr() if need else None, need)
+    if r:
+        check(r, what)
     return out
 
 

@@ -114,7 +114,7 @@ def test_row_strides(s2lib):
 
 
 def test_operand_strides(s2lib):
-    stride = lambda t: s2lib._operand_stride(t, -1, "t")  # noqa: E731
+    stride = lambda t: s2lib._operand_stride(t, t.shape, -1, "t")  # noqa: E731
     rows = lambda *shape: torch.empty(shape, dtype=torch.bfloat16)  # noqa: E731
     assert stride(rows(4, 16)) == 16 and stride(rows(4, 24)[:, :13]) == 24
     assert stride(rows(1, 13)) == 16 and stride(rows(4, 24)[2:3, :13]) == 16, "a row of its own has no stride"
