@@ -360,7 +360,9 @@ __device__ __forceinline__ void st_cluster_v4(uint32_t addr, float4 v)
 }
 
 // ---------------------------------------------------------------- slab kernel
-constexpr int kHeld = 8; // rows of its vector column per thread, in registers
+// Rows of its vector column per thread, in registers: two forms of the kernel,
+// since the longer one's code costs a small x 0.3 us.
+constexpr int kHeld = 8, kHeldMost = 12;
 
 // Bytes of the reduction: units x pitch.
 size_t red_bytes(int cols, int per_thread)
@@ -373,10 +375,9 @@ size_t slab_smem(int cluster, int groups, int cols, int per_thread)
     return (size_t)(cluster + 1) * groups * 16 + (size_t)groups * 8 + red_bytes(cols, per_thread);
 }
 
-template <typename TI, typename TO, int V>
+template <typename TI, typename TO, int V, int K>
 __global__ void __launch_bounds__(kThreads, 1) group_norm_slab_kernel(const GroupNormArgs a)
 {
-    constexpr int K = kHeld;
     extern __shared__ __align__(16) uint8_t smem[];
     const int G = a.groups, P = a.parts;
     float4* table = reinterpret_cast<float4*>(smem); // [P][G], written by the cluster
@@ -749,23 +750,29 @@ int widest_slice(int C, int unit, int most)
 
 struct Cut
 {
-    bool slab;
+    int held; // rows a thread of the slab kernel holds, 0: sums and apply
     int slice, parts;
 };
 
 // How a problem is cut for vectors of V channels (16 or 8 bytes, or 1 where
 // groups, strides or bases do not admit them).
-//   Slab kernel: slices of 64 bytes (more CTAs; 256 x 512 bf16 4.7 us, against
-//   5.0 in slices of 128 bytes and 5.5 with clusters of 8), clusters as small
-//   as hold the rows, and only where all of it is resident at once (two CTAs a
-//   SM): 4,096 x 512 takes 8.1 us so and 11.2 in two kernels, but a second
-//   wave costs what a second kernel does.
+//   Slab kernel: slices of 64 bytes (more CTAs; 256 x 512 bf16 4.5 us, against
+//   5.0 in slices of 128 bytes and 5.5 with clusters of 8), 8 rows a thread,
+//   clusters as small as hold the rows, and only where all of it is resident at
+//   once: two CTAs a SM for clusters of up to 8 (4,096 x 512 takes 7.7 us so and
+//   11.2 in two kernels), fewer for larger ones, which find less room (6,000 x
+//   512: 8.2 us in clusters of 12, 192 CTAs, 13.1 in clusters of 16; 7,000 x 512
+//   13.6 in clusters of 14, 224 CTAs).  What does not fit so gets up to 12 rows
+//   a thread with the same bound (7,000 x 512 9.0 us, 9,000 x 512 9.7 against
+//   11.7 in two kernels, 4 x 4,400 x 256 8.8 against 12.9; 3 x 3,555 x 320 fp32,
+//   288 CTAs, would take 17.7 against 11.0).
 //   Sums and apply: slices of at most 128 channels, one wave of CTAs (6 x
 //   14,400 x 512 bf16: 45.5 us at 444 parts, 49.9 at 296, 52.8 at 888).
-constexpr int kSlabCtas = 2 * 148;
+constexpr int kSlabCtas = 2 * 148, kLongCtas = 192;
 constexpr int kPartCtas = kBlocks * 148;
 // Values a CTA at least: with fewer its set-up costs more than it saves (6 x
-// 4,282 x 128 17.7 us at 8,192, 15.0 at 16,384; 1 x 53,217 x 33 12.3 and 14.7).
+// 4,282 x 128 in two kernels 17.7 us at 8,192, 15.0 at 16,384; 1 x 53,217 x 33
+// 12.3 and 14.7).
 constexpr int kPartMin = 16384;
 
 Cut cut(int64_t instances, int64_t rows, int C, int width, int V)
@@ -774,12 +781,19 @@ Cut cut(int64_t instances, int64_t rows, int C, int width, int V)
     c.slice = widest_slice(C, width / gcd(width, V) * V, V > 1 ? 4 * V : 32);
     if (c.slice / V <= kThreads)
     {
-        const int64_t held = (int64_t)(kThreads / (c.slice / V)) * kHeld; // rows a CTA holds
-        c.parts = 1;
-        while (c.parts < kMaxCluster && c.parts * held < rows) c.parts *= 2;
-        c.slab = c.parts * held >= rows && instances * (C / c.slice) * c.parts <= kSlabCtas;
+        const int64_t slots = kThreads / (c.slice / V), slabs = instances * (C / c.slice);
+        int64_t p = 1, fewest = (rows + slots * kHeld - 1) / (slots * kHeld);
+        while (p < fewest && p < 8) p *= 2;
+        p = std::max(p, fewest);
+        if (p <= kMaxCluster && slabs * p <= (p > 8 ? kLongCtas : kSlabCtas)) c.held = kHeld;
+        if (!c.held)
+        {
+            p = (rows + slots * kHeldMost - 1) / (slots * kHeldMost);
+            if (p <= kMaxCluster && slabs * p <= kLongCtas) c.held = kHeldMost;
+        }
+        c.parts = (int)p; // of the slab kernel
     }
-    if (!c.slab)
+    if (!c.held)
     {
         // the same slices for every V that vectors_fit() admits: multiples of 8
         // channels where these fit the row, else of 4, else single groups
@@ -850,18 +864,21 @@ int launch(Context& ctx, GroupNormArgs a, int instances, int C, void* workspace)
     a.by_width = (uint32_t)(((1ull << 32) + a.width - 1) / a.width);
     const int64_t grid = (int64_t)instances * a.slices * a.parts;
     ProfileScope prof(ctx, K_NORM, 0.0, (double)instances * a.rows * C * (sizeof(TI) + sizeof(TO)));
-    if (c.slab)
+    if (c.held)
     {
-        static std::atomic<uint64_t> seen{0};
-        return launch_kernel(ctx, group_norm_slab_kernel<TI, TO, V>, seen, grid, a.parts,
-                             slab_smem(a.parts, a.groups, cols, V / a.sub), false, a);
+        static std::atomic<uint64_t> seen{0}, seen_long{0};
+        const size_t smem = slab_smem(a.parts, a.groups, cols, V / a.sub);
+        if (c.held == kHeld)
+            return launch_kernel(ctx, group_norm_slab_kernel<TI, TO, V, kHeld>, seen, grid, a.parts, smem, false, a);
+        return launch_kernel(ctx, group_norm_slab_kernel<TI, TO, V, kHeldMost>, seen_long, grid, a.parts, smem, false, a);
     }
     a.partial = static_cast<float2*>(workspace);
     static std::atomic<uint64_t> seen_sums{0}, seen_apply{0};
     const int r = launch_kernel(ctx, group_norm_sums_kernel<TI, V>, seen_sums, grid, 1,
                                 (size_t)a.groups * 16 + red_bytes(cols, V / a.sub) + kRingBytes<TI, V>, false, a);
     if (r != S2_OK) return r;
-    return launch_kernel(ctx, group_norm_apply_kernel<TI, TO, V>, seen_apply, grid, 1, ((size_t)a.groups * 8 + 15) / 16 * 16 + kRingBytes<TI, V>, true, a);
+    return launch_kernel(ctx, group_norm_apply_kernel<TI, TO, V>, seen_apply, grid, 1,
+                         ((size_t)a.groups * 8 + 15) / 16 * 16 + kRingBytes<TI, V>, true, a);
 }
 
 // Vectors of V channels: whole ones in a row's groups, at aligned addresses.
@@ -896,7 +913,7 @@ size_t s2_group_norm_workspace(int instances, int64_t rows, int channels, int gr
     for (int V : {8, 4, 1}) // whatever the type and alignment turn out to be
     {
         const s2::Cut c = s2::cut(instances, rows, channels, channels / groups, V);
-        if (!c.slab) need = std::max(need, (size_t)instances * groups * c.parts * sizeof(float2));
+        if (!c.held) need = std::max(need, (size_t)instances * groups * c.parts * sizeof(float2));
     }
     return need;
 }

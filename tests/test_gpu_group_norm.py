@@ -49,6 +49,21 @@ def test_group_norm(s2lib, gpu_ctx, size, form):
     oracles.check(got, *oracles.group_norm(x, g, gamma, beta, 1e-5, act, DT[tout]), f"{size} {form}")
 
 
+@pytest.mark.parametrize("size", [(6, 4282, 128, 32), (1, 6000, 512, 32), (1, 5001, 512, 32), (1, 12288, 512, 32),
+                                  (1, 4000, 33, 33), (1, 6100, 36, 4), (2, 6529, 20, 1)], ids=str)
+@pytest.mark.parametrize("types", [("bf16", "bf16"), ("f32", "bf16"), ("bf16", "f32"), ("f32", "f32")],
+                         ids=lambda t: "-".join(t))
+def test_clusters_of_any_size(s2lib, gpu_ctx, size, types):
+    """Rows that more than eight a thread of a cluster hold."""
+    i, r, c, g = size
+    x = _x(r + c, i, r, c, DT[types[0]])
+    gamma, beta = _affine(c, c)
+    got = s2lib.group_norm(gpu_ctx, x, g, gamma, beta, act=s2lib.S2_ACT_SILU,
+                           out_dtype=s2lib.S2_DTYPE_F32 if types[1] == "f32" else s2lib.S2_DTYPE_BF16)
+    assert gpu_ctx.status() == 0
+    oracles.check(got, *oracles.group_norm(x, g, gamma, beta, 1e-6, "silu", DT[types[1]]), f"{size} {types}")
+
+
 def test_large_slabs(s2lib, gpu_ctx):
     """More rows than the cluster's shared memory keeps: the rest is read again."""
     for tin, i, r, c, g, far in (("f32", 1, 60000, 128, 32, 1.5), ("bf16", 2, 100000, 64, 2, 30.0)):
