@@ -505,13 +505,11 @@ def _new(ctx, shape, dtype):
     there before, and kept for the work of torch's current stream, where the caller takes it."""
     import torch
 
-    device = torch.device("cuda", ctx.device)
-    current = torch.cuda.current_stream(device)
-    if current == ctx.stream:
-        return torch.empty(shape, device=device, dtype=dtype)
+    if torch._C._cuda_getCurrentRawStream(ctx.device) == ctx.stream.cuda_stream:
+        return torch.empty(shape, device=ctx.device, dtype=dtype)
     with torch.cuda.stream(ctx.stream):
-        t = torch.empty(shape, device=device, dtype=dtype)
-    t.record_stream(current)
+        t = torch.empty(shape, device=ctx.device, dtype=dtype)
+    t.record_stream(torch.cuda.current_stream(ctx.device))
     return t
 
 
