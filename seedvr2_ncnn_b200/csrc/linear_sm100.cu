@@ -24,13 +24,15 @@ constexpr int kMaxGroups = 1024;
 constexpr size_t kSmemLimit = 232448;
 
 // The tensor core adds into its fp32 accumulator without rounding to nearest:
-// an fp32 result is off by 6e-8 of itself for each K block in one sum (1.2e-5
+// an fp32 result is off by 6.2e-8 of itself for each K block in one sum (1.1e-5
 // over K = 10,240).  Where the result is fp32, sums of at most kChunk blocks
-// (9e-7) are therefore added up in fp32 registers (or shared memory), each while
-// the tensor core works on the next one: 21,658 x 2,560 x 10,240 takes 898 us so
-// (869 at 24 blocks, 916 at 12) and 835 in one sum.  A bf16 result rounds at
-// 2^-9 and keeps one sum.
-constexpr int kChunk = 16;
+// (8.7e-7, so that an activation's slope keeps it below 1e-6) are therefore
+// added up in fp32 registers (or shared memory), each while the tensor core
+// works on the next one: 21,658 x 2,560 x 10,240 with an fp32 residual takes 886
+// us so (860 at 24 blocks, 920 at 12) and 810 in one sum.  The price is highest
+// where K just passes one sum: x 1,024 236 us against 156.  A bf16 result rounds
+// at 2^-9 and keeps one sum.
+constexpr int kChunk = 14;
 
 // Blocks of one sum: equal ones.
 constexpr int chunk_blocks(int num_kb, bool out_f32)
@@ -181,6 +183,11 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity)
 }
 
 // ---------------------------------------------------------------- many rows
+// Bound by the tensor core: 21,658 x 7,680 x 2,560 in two groups takes 559 us =
+// 1,523 TFLOP/s of the 1,701 that a library product reaches at full clock (682 us
+// where power holds the clock down).  Short K is bound by memory and by the
+// epilogue that shares it: 288,000 x 256 x 512 with a residual 111 us = 5.3 TB/s
+// of 6.45.
 // Warps: TMA, MMA, then EW for the epilogue, in equal parts over the four TMEM
 // lane quarters, each with its share of the columns.  Eight do where boxes
 // leave by TMA; sixteen where the warps copy them, a chain of latencies that
@@ -889,7 +896,9 @@ __global__ void __launch_bounds__(tile_threads(EW, SUM), 1)
 // partial sums in its shared memory, and after a cluster barrier CTA r adds
 // the S parts of rows r, r + S, ... in rank order (the result does not depend
 // on the run), applies the epilogue and stores: a warp takes one row's 128
-// features, four a lane.
+// features, four a lane.  1 x 2,560 x 2,560 takes 7.0 us (2.0 at the memory's
+// rate: the set-up, one trip to memory and two cluster barriers are the rest), 58 x
+// 10,240 x 2,560 16.0 (8.4), 64 groups of 2,048 x 1,024 at 2 rows 37 = 5.3 TB/s.
 constexpr int kRowsThreads = 192;
 
 template <int TN>

@@ -154,8 +154,8 @@ def test_grouped_linear_long_sums(s2lib, gpu_ctx, layout, n):
 
 @pytest.mark.parametrize("rows", [1, 40, 300, 2500])
 def test_fp32_results_keep_their_precision(s2lib, gpu_ctx, rows):
-    """K = 10,240 without a residual: the 2-norm of the error stays at 2e-6 of the result's (sums of 16 blocks of 64
-    lose 16 steps of 4 products' worth, some 6e-8 a block, whatever K is; one sum of 160 blocks lost 1.2e-5)."""
+    """K = 10,240 without a residual: the 2-norm of the error stays at 2e-6 of the result's (sums of 14 blocks of 64
+    lose some 6e-8 a block, whatever K is; one sum of 160 blocks lost 1.1e-5)."""
     a, w, _, _, _ = _case(9, rows, 384, 10240, bias=False, out="f32")
     got = s2lib.linear(gpu_ctx, a, w, out_dtype=s2lib.S2_DTYPE_F32).double()
     want = a.double() @ w.double().t()
