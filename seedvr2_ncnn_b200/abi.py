@@ -611,10 +611,9 @@ def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=
     out_code = codes.get(out.dtype)
     if out_code is None or out.shape != shape or out.get_device() != dev:
         _refuse(what)
-    if gamma is not None:
-        gamma = _vector(gamma, shape[-1:], dev, what)
-    if beta is not None:
-        beta = _vector(beta, shape[-1:], dev, what)
+    # under names of their own: a tensor that only this call holds would free its memory to the workspace
+    gamma_at = None if gamma is None else _vector(gamma, shape[-1:], dev, what)
+    beta_at = None if beta is None else _vector(beta, shape[-1:], dev, what)
     L = lib()
     need = L.s2_group_norm_workspace(instances, rows, channels, groups)
     ws = None
@@ -622,8 +621,8 @@ def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=
         import torch
 
         ws = _new(ctx, need, torch.uint8)
-    r = L.s2_group_norm(ctx.handle, instances, rows, channels, groups, code, x.data_ptr(), _row_stride(x, what), gamma,
-                        beta, eps, act, out_code, out.data_ptr(), _row_stride(out, what),
+    r = L.s2_group_norm(ctx.handle, instances, rows, channels, groups, code, x.data_ptr(), _row_stride(x, what),
+                        gamma_at, beta_at, eps, act, out_code, out.data_ptr(), _row_stride(out, what),
                         ws.data_ptr() if need else None, need)
     if r:
         check(r, what)
