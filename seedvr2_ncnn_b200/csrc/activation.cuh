@@ -1,13 +1,14 @@
 // Activations of the linear and group norm epilogues (S2_ACT_*), on fp32
 // values held as pairs (packed f32x2 arithmetic).
 //
-// Exact form: x sigmoid(t) = x / (1 + e^-t).  No cancellation, so the error
-// stays at a few units of 2^-24 of the result, where an fp32 output keeps it.
-// Four values share one reciprocal -- 1/a = b c d / (a b c d) -- so a value
-// costs 1.25 special-function operations instead of 2 (an SM starts 16 a
-// clock).  For that t is held at -21 and above, which keeps the product of
-// four finite: further out the result is below 1e-9 |x| either way.  A NaN t
-// becomes -21 there, so a NaN value reaches only itself.
+// Exact form: x sigmoid(t), sigmoid(t) = (t < 0 ? u : 1) / (1 + u) with
+// u = e^-|t| <= 1.  No cancellation, so the error stays at a few units of 2^-24
+// of the result, where an fp32 output keeps it, for any t: it goes to zero with
+// u (below 2^-126 u is zero, and so is the result), and at -inf it is the NaN of
+// -inf times zero.  Four values share one reciprocal -- 1/a = b c d / (a b c d),
+// the denominators lie in [1, 2] -- so a value costs 1.25 special-function
+// operations instead of 2 (an SM starts 16 a clock).  A NaN t gives u = 2^-127
+// there, so a NaN value reaches only itself.
 //
 // Fast form, for bf16 results: sigmoid(t) = (1 + tanh(t / 2)) / 2 with
 // tanh.approx, one special-function operation and no reciprocal.  Its error of
@@ -47,9 +48,9 @@ __device__ __forceinline__ float2 splat(float v)
     return make_float2(v, v);
 }
 
-constexpr float kSqrt2OverPi = 0.7978845608028654f;
-constexpr float kGeluCubic = 0.044715f;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kSqrt2OverPi = 0.7978845608028654;
+constexpr double kGeluCubic = 0.044715;
+constexpr double kLog2e = 1.4426950408889634;
 
 // 0.5 x (1 + erf(x / sqrt 2)) without a branch (erff's two branches cost a warp
 // both, one element after another): with z = |x| / sqrt 2 and q = erfc(z) / 2,
@@ -67,7 +68,7 @@ __device__ __forceinline__ float2 gelu_erf(float2 x)
     p = __ffma2_rn(t, p, splat(0.5f * -0.284496736f));
     p = __ffma2_rn(t, p, splat(0.5f * 0.254829592f));
     p = __fmul2_rn(t, p);
-    const float2 z2 = __fmul2_rn(__fmul2_rn(a, splat(-0.5f * kLog2e)), a);
+    const float2 z2 = __fmul2_rn(__fmul2_rn(a, splat((float)(-0.5 * kLog2e))), a);
     p = __fmul2_rn(__fmul2_rn(p, a), make_float2(ex2_approx(z2.x), ex2_approx(z2.y)));
     return make_float2(fmaf(0.5f, x.x + ax.x, -p.x), fmaf(0.5f, x.y + ax.y, -p.y));
 }
@@ -87,21 +88,23 @@ __device__ __forceinline__ void activate(float2 (&v)[N])
 #pragma unroll
         for (int j = 0; j < N; j += H)
         {
-            float2 a[2] = {splat(1.f), splat(1.f)}; // 1 + e^-t
+            float2 a[2] = {splat(1.f), splat(1.f)}; // 1 + u
 #pragma unroll
             for (int i = 0; i < H; i++)
             {
                 const float2 x = v[j + i];
                 float2 t; // -t log2(e)
                 if constexpr (ACT == S2_ACT_SILU)
-                    t = __fmul2_rn(x, splat(-kLog2e));
+                    t = __fmul2_rn(x, splat((float)-kLog2e));
                 else
                 {
-                    // 0.5 x (1 + tanh(u)) = x sigmoid(2u), u = sqrt(2/pi) (x + 0.044715 x^3)
-                    const float k = -2.f * kLog2e * kSqrt2OverPi;
-                    t = __fmul2_rn(x, __ffma2_rn(__fmul2_rn(x, splat(k * kGeluCubic)), x, splat(k)));
+                    // 0.5 x (1 + tanh(w)) = x sigmoid(2w), w = sqrt(2/pi) (x + 0.044715 x^3)
+                    constexpr double k = -2 * kLog2e * kSqrt2OverPi; // each factor rounded once
+                    t = __fmul2_rn(x, __ffma2_rn(__fmul2_rn(x, splat((float)(k * kGeluCubic))), x, splat((float)k)));
                 }
-                a[i] = __fadd2_rn(make_float2(ex2_approx(fminf(t.x, 30.3f)), ex2_approx(fminf(t.y, 30.3f))), splat(1.f));
+                const float2 u = make_float2(ex2_approx(-fminf(fabsf(t.x), 127.f)), ex2_approx(-fminf(fabsf(t.y), 127.f)));
+                a[i] = __fadd2_rn(u, splat(1.f));
+                v[j + i] = __fmul2_rn(x, make_float2(t.x > 0.f ? u.x : 1.f, t.y > 0.f ? u.y : 1.f));
             }
             const float ab = a[0].x * a[0].y, cd = a[1].x * a[1].y;
             const float r = rcp_approx(ab * cd);
@@ -134,7 +137,7 @@ __device__ __forceinline__ void activate_fast(float2 (&h)[N])
         {
             float2 t = h[j];
             if constexpr (ACT == S2_ACT_GELU_TANH)
-                t = __fmul2_rn(t, __ffma2_rn(__fmul2_rn(t, splat(8.f * kSqrt2OverPi * kGeluCubic)), t, splat(2.f * kSqrt2OverPi)));
+                t = __fmul2_rn(t, __ffma2_rn(__fmul2_rn(t, splat((float)(8 * kSqrt2OverPi * kGeluCubic))), t, splat((float)(2 * kSqrt2OverPi))));
             h[j] = __ffma2_rn(h[j], make_float2(tanh_of(t.x), tanh_of(t.y)), h[j]);
         }
     }
