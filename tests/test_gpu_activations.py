@@ -25,9 +25,17 @@ def _values():
 
 def _want(x, act, dtype):
     """(act(x), bound) of the formula in 64 bits.  Beside what oracles.activated() counts of the sigmoid forms: a
-    sigmoid below 2^-126 is zero."""
+    sigmoid below 2^-126 is zero.
+
+    GELU with erf is max(x, 0) - a q, a = |x|, q = erfc(a / sqrt 2) / 2 = r P(6 r - 1) exp(-a^2 / 2), r = 1 / (a + 3).
+    Relative to q in units of U: r 3 (a sum, a reciprocal of one ulp), which counts 1 + 6 r P' / P <= 2.4 times, 7; the
+    argument of P rounded once, times P' / P, 1; P's own steps 3 and its fit 1; the exponent's three roundings
+    3 a^2 / 2, the exponential 4 (two ulp); two products and one with a 3.  Together 19 + 1.5 a^2; then the sum."""
     x = x.double()
     y, bound = oracles.activated(x, torch.zeros_like(x), act)
+    if act == "gelu_erf":
+        a = x.abs().clamp(max=40)
+        bound = (20 + 2 * a**2) * U * a * torch.special.erfc(a / math.sqrt(2)) / 2 + 2 * U * y.abs()
     bound = bound + 2.0**-126 * x.abs()
     return y, bound + oracles.half_step(dtype) * (y.abs() + bound) + 1e-37
 
@@ -41,7 +49,7 @@ def _check(got, x, act, dtype, what):
     assert torch.equal(got.double()[inf], want[inf]), f"{what}: other infinities"
 
 
-ACTS = ["silu", "gelu_tanh"]
+ACTS = ["silu", "gelu_tanh", "gelu_erf"]
 
 # rows, K: the transposed product, single CTAs, CTA pairs; with fp32 results the two K of 15 blocks sum in registers
 LINEAR = [(1, 8), (40, 8), (700, 8), (6000, 8), (700, 960), (6000, 960)]
