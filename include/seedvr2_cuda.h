@@ -257,9 +257,8 @@ int s2_grouped_linear(s2_context* ctx, int rows, int groups, const int* offsets,
  * with the same type and stride; otherwise they do not overlap.  gamma, beta:
  * fp32 [channels] or NULL.  channels is a multiple of groups; rows <= 2^30.
  * channels <= 65536; 16-byte aligned bases and row strides are fastest.  NaN or
- * Inf in a group makes that group's results NaN and no other's.  Activations of
- * a bf16 result are within |z| 2^-12 of act(z) before its rounding.  The same
- * call gives the same bits; it may be captured.
+ * Inf in a group makes that group's results NaN and no other's.  The same call
+ * gives the same bits; it may be captured.
  * workspace: s2_group_norm_workspace bytes (0 for small x, then NULL will do),
  * 8-byte aligned, contents irrelevant before and after; calls that may run at
  * the same time need one each. */

@@ -1,19 +1,18 @@
 // Activations of the linear and group norm epilogues (S2_ACT_*), on fp32
 // values held as pairs (packed f32x2 arithmetic).
 //
-// Exact form: x sigmoid(t), sigmoid(t) = (t < 0 ? u : 1) / (1 + u) with
-// u = e^-|t| <= 1.  No cancellation, so the error stays at a few units of 2^-24
-// of the result, where an fp32 output keeps it, for any t: it goes to zero with
-// u (below 2^-126 u is zero, and so is the result), and at -inf it is the NaN of
-// -inf times zero.  Four values share one reciprocal -- 1/a = b c d / (a b c d),
-// the denominators lie in [1, 2] -- so a value costs 1.25 special-function
-// operations instead of 2 (an SM starts 16 a clock).  A NaN t gives u = 2^-127
-// there, so a NaN value reaches only itself.
+// x sigmoid(t) = x / (1 + e^-t): no cancellation, so the error stays at a few
+// units of 2^-24 of the result for any t, bf16 results included: what is rounded
+// to bf16 is far smaller than x where x is negative, and an absolute error of x's
+// size would show.  Further out e^-t becomes infinite and the result zero; at
+// -inf it is the NaN of -inf times zero.
 //
-// Fast form, for bf16 results: sigmoid(t) = (1 + tanh(t / 2)) / 2 with
-// tanh.approx, one special-function operation and no reciprocal.  Its error of
-// 2^-11 leaves |x| 2^-12, a sixteenth of the half step that rounding x itself
-// to bf16 would cost.
+// Two special-function operations a value (an SM starts 16 a clock) and little
+// else.  Four values that share one reciprocal need 1.25, and seven instructions
+// more for products and for an exponent that stays in range: 8,000 x 2,560 x
+// 1,024 with fp32 results and tanh GELU 76 us so and 88 shared, 6 x 14,400 x 512
+// group norm with SiLU 55 and 55, but 60,000 x 1,024 x 256 in bf16 with SiLU 86
+// and 80.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -33,13 +32,6 @@ __device__ __forceinline__ float ex2_approx(float x)
 {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ float tanh_of(float x)
-{
-    float y;
-    asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -79,7 +71,7 @@ __device__ __forceinline__ float2 gelu_erf(float2 x)
     return make_float2(fmaf(0.5f, x.x + ax.x, -p.x), fmaf(0.5f, x.y + ax.y, -p.y));
 }
 
-// v = act(v), exact form
+// v = act(v)
 template <int ACT, int N>
 __device__ __forceinline__ void activate(float2 (&v)[N])
 {
@@ -90,68 +82,26 @@ __device__ __forceinline__ void activate(float2 (&v)[N])
     }
     else if constexpr (ACT != S2_ACT_NONE)
     {
-        constexpr int H = N % 2 == 0 ? 2 : 1; // pairs that share a reciprocal
-#pragma unroll
-        for (int j = 0; j < N; j += H)
-        {
-            float2 a[2] = {splat(1.f), splat(1.f)}; // 1 + u
-#pragma unroll
-            for (int i = 0; i < H; i++)
-            {
-                const float2 x = v[j + i];
-                float2 t; // -t log2(e)
-                if constexpr (ACT == S2_ACT_SILU)
-                    t = __fmul2_rn(x, splat((float)-kLog2e));
-                else
-                {
-                    // 0.5 x (1 + tanh(w)) = x sigmoid(2w), w = sqrt(2/pi) (x + 0.044715 x^3)
-                    constexpr double k = -2 * kLog2e * kSqrt2OverPi; // each factor rounded once
-                    t = __fmul2_rn(x, __ffma2_rn(__fmul2_rn(x, splat((float)(k * kGeluCubic))), x, splat((float)k)));
-                }
-                const float2 u = make_float2(ex2_approx(-fminf(fabsf(t.x), 127.f)), ex2_approx(-fminf(fabsf(t.y), 127.f)));
-                a[i] = __fadd2_rn(u, splat(1.f));
-                v[j + i] = __fmul2_rn(x, make_float2(t.x > 0.f ? u.x : 1.f, t.y > 0.f ? u.y : 1.f));
-            }
-            const float ab = a[0].x * a[0].y, cd = a[1].x * a[1].y;
-            const float r = rcp_approx(ab * cd);
-            const float rab = r * cd, rcd = r * ab;
-            v[j].x *= rab * a[0].y;
-            v[j].y *= rab * a[0].x;
-            if constexpr (H == 2)
-            {
-                v[j + 1].x *= rcd * a[1].y;
-                v[j + 1].y *= rcd * a[1].x;
-            }
-        }
-    }
-}
-
-// Whether the fast form below takes this activation's argument halved.
-constexpr bool fast_halves(int act)
-{
-    return act == S2_ACT_SILU || act == S2_ACT_GELU_TANH;
-}
-
-// h = act(x), fast form, from h = x / 2 where fast_halves(ACT), else from x
-template <int ACT, int N>
-__device__ __forceinline__ void activate_fast(float2 (&h)[N])
-{
-    if constexpr (fast_halves(ACT))
-    {
 #pragma unroll
         for (int j = 0; j < N; j++)
         {
-            float2 t = h[j];
-            if constexpr (ACT == S2_ACT_GELU_TANH)
-                t = __fmul2_rn(t, __ffma2_rn(__fmul2_rn(t, splat((float)(8 * kSqrt2OverPi * kGeluCubic))), t, splat((float)(2 * kSqrt2OverPi))));
-            h[j] = __ffma2_rn(h[j], make_float2(tanh_of(t.x), tanh_of(t.y)), h[j]);
+            const float2 x = v[j];
+            float2 t; // -t log2(e)
+            if constexpr (ACT == S2_ACT_SILU)
+                t = __fmul2_rn(x, splat((float)-kLog2e));
+            else
+            {
+                // 0.5 x (1 + tanh(w)) = x sigmoid(2w), w = sqrt(2/pi) (x + 0.044715 x^3)
+                constexpr double k = -2 * kLog2e * kSqrt2OverPi; // each factor rounded once
+                t = __fmul2_rn(x, __ffma2_rn(__fmul2_rn(x, splat((float)(k * kGeluCubic))), x, splat((float)k)));
+            }
+            const float2 d = __fadd2_rn(make_float2(ex2_approx(t.x), ex2_approx(t.y)), splat(1.f));
+            v[j] = __fmul2_rn(x, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
         }
     }
-    else
-        activate<ACT>(h);
 }
 
-// Exact form of N values, the activation given at run time.
+// The same of N values, the activation given at run time.
 template <int N>
 __device__ __forceinline__ void activate(float (&v)[N], int act)
 {

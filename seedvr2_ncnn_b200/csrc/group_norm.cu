@@ -297,10 +297,8 @@ template <typename TO, int V>
 struct Scale
 {
     float2 neg[kPairs<V>], mul[kPairs<V>], off[kPairs<V>];
-    static constexpr bool FAST = sizeof(TO) == 2;
     __device__ void load(const GroupNormArgs& a, const float2* stat, int c0, int col)
     {
-        const float half = FAST && fast_halves(a.act) ? 0.5f : 1.f; // exact
 #pragma unroll
         for (int j = 0; j < kPairs<V>; j++)
         {
@@ -311,8 +309,8 @@ struct Scale
                 const int c = col * V + 2 * j + h;
                 const float2 t = stat[a.width > 1 ? (int)__umulhi(c, a.by_width) : c]; // (mean, rstd)
                 v[0][h] = -t.x;
-                v[1][h] = t.y * (a.gamma ? __ldg(a.gamma + c0 + c) : 1.f) * half;
-                v[2][h] = a.beta ? __ldg(a.beta + c0 + c) * half : 0.f;
+                v[1][h] = t.y * (a.gamma ? __ldg(a.gamma + c0 + c) : 1.f);
+                v[2][h] = a.beta ? __ldg(a.beta + c0 + c) : 0.f;
             }
             neg[j] = make_float2(v[0][0], v[0][1]);
             mul[j] = make_float2(v[1][0], v[1][1]);
@@ -324,10 +322,7 @@ struct Scale
     {
 #pragma unroll
         for (int j = 0; j < kPairs<V>; j++) f[j] = __ffma2_rn(__fadd2_rn(f[j], neg[j]), mul[j], off[j]);
-        if constexpr (FAST)
-            activate_fast<ACT>(f);
-        else
-            activate<ACT>(f);
+        activate<ACT>(f);
         store_out<TO, V>(out, f);
     }
 };

@@ -88,7 +88,7 @@ NORM = [(1, 5), (2, 700), (1, 6000), (2, 30000)]
 
 
 @pytest.mark.parametrize("tin", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
-@pytest.mark.parametrize("tout", [torch.float32], ids=["to_f32"])
+@pytest.mark.parametrize("tout", [torch.bfloat16, torch.float32], ids=["to_bf16", "to_f32"])
 @pytest.mark.parametrize("instances,rows", NORM)
 @pytest.mark.parametrize("whole", [True, False], ids=["vectors", "single"])
 @pytest.mark.parametrize("act", ACTS)
