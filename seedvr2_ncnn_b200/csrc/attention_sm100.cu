@@ -920,17 +920,18 @@ int launch_window_attention(Context& ctx, const AttnSchedule& s, int heads, cons
     a.status = ctx.status;
     for (int i = 0; i < kMaxPeers; i++) a.peer_out[i] = i < num_peers ? peer_out[i] : nullptr;
     static std::atomic<uint64_t> configured{0};
-    if (first_on_device(configured))
-    {
+    const int set = set_up_current_device(configured, [] {
         // The register split assumes exactly LAUNCH_REGS per thread at launch
         // (a different count would leave the softmax warps' increase waiting).
         cudaFuncAttributes fa;
         if (cudaFuncGetAttributes(&fa, window_attention_kernel) != cudaSuccess || fa.numRegs != LAUNCH_REGS)
-            return S2_ERR_CUDA;
+            return (int)S2_ERR_CUDA;
         if (cudaFuncSetAttribute(window_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) !=
             cudaSuccess)
-            return S2_ERR_CUDA;
-    }
+            return (int)S2_ERR_CUDA;
+        return (int)S2_OK;
+    });
+    if (set != S2_OK) return set;
     a.heads = heads;
     a.num_work = s.num_items * heads;
     a.num_video_indices = s.num_video_indices;

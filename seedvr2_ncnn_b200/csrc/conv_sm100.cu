@@ -418,8 +418,9 @@ int conv3d_gemm(Context& ctx, const Conv3dGeometry& g, const void* X, int frames
     a.status = ctx.status;
     if (a.num_tiles <= 0) return S2_OK;
     static std::atomic<uint64_t> configured{0};
-    if (first_on_device(configured) &&
-        cudaFuncSetAttribute(conv3d_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C_SMEM) != cudaSuccess)
+    if (set_up_current_device(configured, [] {
+            return cudaFuncSetAttribute(conv3d_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C_SMEM);
+        }) != cudaSuccess)
         return S2_ERR_CUDA;
     const int grid = a.num_tiles < ctx.num_sms ? a.num_tiles : ctx.num_sms;
     const double flops = 2.0 * g.Tout * g.Ho * g.Wo * (double)g.Co * taps * g.Ci;

@@ -1365,13 +1365,11 @@ cudaError_t launch_pair_variant(cudaStream_t stream, const CUtensorMap& ta0, con
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (first_on_device(configured))
-    {
-        const cudaError_t e = cudaFuncSetAttribute(shared_linear_pair_kernel<SKB, EK>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   PairTile<SKB, EK>::SMEM_BYTES);
-        if (e != cudaSuccess) return e;
-    }
+    const cudaError_t set = set_up_current_device(configured, [] {
+        return cudaFuncSetAttribute(shared_linear_pair_kernel<SKB, EK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    PairTile<SKB, EK>::SMEM_BYTES);
+    });
+    if (set != cudaSuccess) return set;
     if (max_clusters.load() == 0)
     {
         cfg.gridDim = dim3(2);
@@ -1426,13 +1424,11 @@ cudaError_t launch_variant(int grid, cudaStream_t stream, const CUtensorMap& ta0
                            const CUtensorMap& tw, const CUtensorMap& to0, const CUtensorMap& to1, const GemmArgs& a)
 {
     static std::atomic<uint64_t> configured{0}; // per instantiation and device
-    if (first_on_device(configured))
-    {
-        const cudaError_t e =
-            cudaFuncSetAttribute(shared_linear_kernel<BN, SKB, EK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 Tile<BN, SKB, EK>::SMEM_BYTES);
-        if (e != cudaSuccess) return e;
-    }
+    const cudaError_t set = set_up_current_device(configured, [] {
+        return cudaFuncSetAttribute(shared_linear_kernel<BN, SKB, EK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    Tile<BN, SKB, EK>::SMEM_BYTES);
+    });
+    if (set != cudaSuccess) return set;
     shared_linear_kernel<BN, SKB, EK>
         <<<grid, num_threads(EK), Tile<BN, SKB, EK>::SMEM_BYTES, stream>>>(ta0, ta1, tw, to0, to1, a);
     return cudaGetLastError();

@@ -804,13 +804,12 @@ template <class K>
 int launch_kernel(Context& ctx, K kernel, std::atomic<uint64_t>& configured, int64_t grid, int cluster, size_t smem,
                   bool after, const GroupNormArgs& a)
 {
-    if (grid > 0x7fffffff || smem > 232448) return S2_ERR_INVALID;
-    if (first_on_device(configured))
-    {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess ||
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-            return S2_ERR_CUDA;
-    }
+    if (grid > 0x7fffffff || smem > 200 * 1024) return S2_ERR_INVALID;
+    if (set_up_current_device(configured, [&] {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+            return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        }) != cudaSuccess)
+        return S2_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     int n = 0;

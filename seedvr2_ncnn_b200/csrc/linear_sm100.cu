@@ -1293,15 +1293,15 @@ int launch_tiles(Context& ctx, const Operands& o, const BoxMaps& m, LinearArgs a
 
     static std::atomic<uint64_t> configured{0}; // per instantiation and device
     static std::atomic<int> resident{0};        // CTAs or pairs at once, the same on every B200
-    if (first_on_device(configured))
-    {
+    const int set = set_up_current_device(configured, [&] {
         cudaFuncAttributes f;
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit) != cudaSuccess ||
             cudaFuncGetAttributes(&f, kernel) != cudaSuccess)
-            return S2_ERR_CUDA;
+            return (int)S2_ERR_CUDA;
         // launched with fewer registers, setmaxnreg.inc would wait for good
-        if (SUM && f.numRegs != kLaunchRegs) return S2_ERR_CUDA;
-    }
+        return SUM && f.numRegs != kLaunchRegs ? (int)S2_ERR_CUDA : (int)S2_OK;
+    });
+    if (set != S2_OK) return set;
     cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = cluster_config(attr, CTAS, CTAS, tile_threads(EW, SUM), smem, ctx.stream);
     int most = CTAS == 1 ? ctx.num_sms : resident.load();
@@ -1335,11 +1335,10 @@ int launch_rows_as(Context& ctx, const Operands& o, const LinearArgs& a, int row
         r = make_tmap_bf16_2d(&tw, o.W, a.K, (uint64_t)a.groups * a.N, (uint64_t)o.ldw * 2, BK, 128);
     if (r != S2_OK) return r;
     static std::atomic<uint64_t> configured{0};
-    if (first_on_device(configured))
-    {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RS::SMEM_BYTES) != cudaSuccess)
-            return S2_ERR_CUDA;
-    }
+    if (set_up_current_device(configured, [&] {
+            return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RS::SMEM_BYTES);
+        }) != cudaSuccess)
+        return S2_ERR_CUDA;
     cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = cluster_config(attr, S, (unsigned)(a.groups * a.nblk * S), kRowsThreads, RS::SMEM_BYTES,
                                             ctx.stream);

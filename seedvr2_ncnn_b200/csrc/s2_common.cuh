@@ -9,18 +9,17 @@
 
 #include <atomic>
 
+#include "set_up_once.h"
+
 namespace s2 {
 
-// Host: true the first time it is called for the current device (one bit
-// per device), so per-function attributes such as the dynamic shared-memory
-// limit are set once on every device a process launches on; safe to call
-// from several host threads (setting an attribute twice is harmless).
-inline bool first_on_device(std::atomic<uint64_t>& seen)
+// Host: set_up_once() for the current device.
+template <class F>
+auto set_up_current_device(std::atomic<uint64_t>& done, F set_up) -> decltype(set_up())
 {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return true;
-    const uint64_t bit = 1ull << dev;
-    return (seen.fetch_or(bit) & bit) == 0;
+    int dev = -1;
+    (void)cudaGetDevice(&dev);
+    return set_up_once(done, dev, set_up);
 }
 
 // Device status word codes (first error wins).
