@@ -283,15 +283,6 @@ __device__ __forceinline__ float bf16_round_f32(float x)
     return __bfloat162float(__float2bfloat16_rn(x));
 }
 
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* status)
-{
-    int ok = 0;
-    if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort, status) ? 1 : 0;
-    ok = __shfl_sync(0xffffffffu, ok, 0);
-    __syncwarp();
-    return ok != 0;
-}
-
 __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity)
 {
     const uint64_t t0 = global_timer_ns();
@@ -813,7 +804,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const int last_valid = wk.S_len - (wk.nkv - 1) * TILE;
             const int nfull = last_valid == TILE ? wk.nkv : wk.nkv - 1;
             auto wait_s = [&]() {
-                if (!warp_wait(&s_full[x], scnt & 1, abort_flag, args.status)) return false;
+                if (!mbar_wait_warp(&s_full[x], scnt & 1, abort_flag, args.status)) return false;
                 scnt++;
                 tc_fence_after();
                 return true;
@@ -846,7 +837,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 softmax_tile<false>(s_addr, o_addr, last_valid, nfull == 0, args.scale_log2, m_used, l_run);
                 release_p();
             }
-            if (!warp_wait(&o_done[x], ocnt & 1, abort_flag, args.status))
+            if (!mbar_wait_warp(&o_done[x], ocnt & 1, abort_flag, args.status))
             {
                 ok = false;
                 break;

@@ -221,11 +221,7 @@ __global__ void __launch_bounds__(C_THREADS, 1)
         uint32_t acc_phase = 0;
         for (int t = blockIdx.x; t < args.num_tiles; t += gridDim.x)
         {
-            int ok = 0;
-            if (lane == 0) ok = mbar_wait<true>(&tfull[acc], acc_phase, abort_flag, args.status) ? 1 : 0;
-            ok = __shfl_sync(0xffffffffu, ok, 0);
-            if (!ok) break;
-            __syncwarp();
+            if (!mbar_wait_warp<true>(&tfull[acc], acc_phase, abort_flag, args.status)) break;
             tc_fence_after();
             int to, y0, x0, n0;
             conv_decode(args, t, to, y0, x0, n0);

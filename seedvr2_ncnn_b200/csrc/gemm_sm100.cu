@@ -736,15 +736,8 @@ __device__ __forceinline__ bool epilogue_gate_residual(const GemmArgs& a, const 
     bool ok = true;
     for (int t = wk.first(); t < a.num_tiles && ok; t += wk.step())
     {
-        int w = 0;
-        if (lane == 0) w = mbar_wait<true>(&tfull[acc], acc_phase, abort_flag, a.status) ? 1 : 0;
-        w = __shfl_sync(0xffffffffu, w, 0);
-        if (!w)
-        {
-            ok = false;
-            break;
-        }
-        __syncwarp();
+        ok = mbar_wait_warp<true>(&tfull[acc], acc_phase, abort_flag, a.status);
+        if (!ok) break;
         tc_fence_after();
         int stream, m0, n0;
         const int width = wk.template decode<BN>(a, t, stream, m0, n0);
@@ -755,14 +748,8 @@ __device__ __forceinline__ bool epilogue_gate_residual(const GemmArgs& a, const 
         for (int c0 = 0; c0 < width && n0 + c0 < N; c0 += 32, q++)
         {
             const int slot = q % R;
-            int r = 0;
-            if (lane == 0) r = mbar_wait<true>(&rfull[slot], (uint32_t)(q / R) & 1u, abort_flag, a.status) ? 1 : 0;
-            r = __shfl_sync(0xffffffffu, r, 0);
-            if (!r)
-            {
-                ok = false;
-                break;
-            }
+            ok = mbar_wait_warp<true>(&rfull[slot], (uint32_t)(q / R) & 1u, abort_flag, a.status);
+            if (!ok) break;
             uint8_t* srow = stg + slot * 4096 + lane * 128;
             const int n = n0 + c0;
             const bool full = n + 32 <= N;
@@ -1014,11 +1001,7 @@ __global__ void __launch_bounds__(num_threads(EK), 1)
             uint32_t acc_phase = 0;
             for (int t = blockIdx.x; t < args.num_tiles; t += gridDim.x)
             {
-                int ok = 0;
-                if (lane == 0) ok = mbar_wait<true>(&tfull[acc], acc_phase, abort_flag, args.status) ? 1 : 0;
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-                if (!ok) break;
-                __syncwarp();
+                if (!mbar_wait_warp<true>(&tfull[acc], acc_phase, abort_flag, args.status)) break;
                 tc_fence_after();
                 int stream, m0, n0;
                 decode_tile<BN>(args, t, stream, m0, n0);
@@ -1290,11 +1273,7 @@ __global__ void __launch_bounds__(num_threads(EK), 1)
             uint32_t acc_phase = 0;
             for (int t = walk.first(); t < args.num_tiles; t += walk.step())
             {
-                int ok = 0;
-                if (lane == 0) ok = mbar_wait<true>(&tfull[acc], acc_phase, abort_flag, args.status) ? 1 : 0;
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-                if (!ok) break;
-                __syncwarp();
+                if (!mbar_wait_warp<true>(&tfull[acc], acc_phase, abort_flag, args.status)) break;
                 tc_fence_after();
                 int khalf;
                 unit_tile(args, t, khalf);

@@ -517,12 +517,9 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
     int q = 0, acc = 0;
     uint32_t acc_phase = 0;
     auto wait_acc = [&]() {
-        int w = 0;
-        if (lane == 0) w = mbar_wait<true>(&tfull[acc], acc_phase, abort_flag, a.status) ? 1 : 0;
-        w = __shfl_sync(0xffffffffu, w, 0);
-        __syncwarp();
+        const bool w = mbar_wait_warp<true>(&tfull[acc], acc_phase, abort_flag, a.status);
         tc_fence_after();
-        return w != 0;
+        return w;
     };
     auto release_acc = [&]() {
         tc_fence_before();
@@ -553,13 +550,7 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
         auto open_box = [&](int c) {
             const int slot = q % R;
             uint8_t* box = stg + slot * kBox;
-            if (a.tma_res)
-            {
-                int r = 0;
-                if (lane == 0) r = mbar_wait<true>(&rfull[slot], (uint32_t)(q / R) & 1u, abort_flag, a.status) ? 1 : 0;
-                r = __shfl_sync(0xffffffffu, r, 0);
-                return r != 0;
-            }
+            if (a.tma_res) return mbar_wait_warp<true>(&rfull[slot], (uint32_t)(q / R) & 1u, abort_flag, a.status);
             if (lane == 0) bulk_wait_read<R - 1>(); // this slot's previous store has read it
             __syncwarp();
             if (copied)
@@ -1187,11 +1178,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
             const int f = (warp & 3) * 32 + lane;
             for (int c0 = kb0; c0 < kb1; c0 += args.chunk_kb)
             {
-                int ok = 0;
-                if (lane == 0) ok = mbar_wait<true>(&tfull[acc], acc_phase, abort_flag, args.status) ? 1 : 0;
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-                if (!ok) break;
-                __syncwarp();
+                if (!mbar_wait_warp<true>(&tfull[acc], acc_phase, abort_flag, args.status)) break;
                 tc_fence_after();
                 const uint32_t t_row = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * RS::ACC_COLS;
 #pragma unroll 1

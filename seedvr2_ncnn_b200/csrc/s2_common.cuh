@@ -147,6 +147,19 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     }
 }
 
+// The same for a whole warp, one lane of which waits.  The shuffle tells the
+// others the answer but orders no memory: __syncwarp() lets them read what the
+// barrier stands for.
+template <bool SLEEP = false>
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int* status)
+{
+    int ok = 0;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait<SLEEP>(bar, parity, abort, status) ? 1 : 0;
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    __syncwarp();
+    return ok != 0;
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const void* desc)
 {
