@@ -1035,6 +1035,45 @@ __device__ __forceinline__ void rows_finish(const LinearArgs& a, const float* pa
     }
 }
 
+// Row tile j of those behind the first of their groups, in the groups' order:
+// its group and its number there (0 if there are fewer).  Each warp looks by
+// itself, a lane over a run of groups.
+template <int TN>
+__device__ __forceinline__ int find_row_tile(const LinearArgs& a, int j, int& group)
+{
+    const int lane = threadIdx.x & 31;
+    const int run = (a.groups + 31) / 32, first = lane * run;
+    auto at = [&](int g) { return max(0, min(__ldg(a.offsets + min(g, a.groups)), a.rows)); };
+    int own = 0;
+    for (int i = 0, lo = at(first); i < run; i++)
+    {
+        const int hi = at(first + i + 1);
+        own += max(0, hi - lo - 1) / TN;
+        lo = hi;
+    }
+    int upto = own;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1)
+    {
+        const int o = __shfl_up_sync(0xffffffffu, upto, m);
+        if (lane >= m) upto += o;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, j < upto);
+    if (!past) return 0;
+    const int owner = __ffs(past) - 1;
+    int g = first, left = j - (upto - own);
+    if (lane == owner)
+        for (int i = 0, lo = at(g); i < run; i++, g++)
+        {
+            const int hi = at(g + 1), more = max(0, hi - lo - 1) / TN;
+            if (left < more) break;
+            left -= more;
+            lo = hi;
+        }
+    group = __shfl_sync(0xffffffffu, g, owner);
+    return 1 + __shfl_sync(0xffffffffu, left, owner);
+}
+
 template <int TN, int S>
 __global__ void __launch_bounds__(kRowsThreads, 2)
     linear_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
@@ -1043,20 +1082,38 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     using RS = RowsShape<TN>;
     constexpr int STAGES = RS::STAGES;
     const int rank = S > 1 ? (int)cluster_ctarank() : 0;
+    // Units: row tiles, each over the blocks of 128 features.  With offsets: each
+    // group's first row tile, then some CTAs (or clusters) that share the others,
+    // whose number the host does not know, in turn.  What they find is the same in
+    // every CTA of a cluster; without rows they return at once.
     const int unit = blockIdx.x / S;
-    const int group = args.groups > 1 ? unit / args.nblk : 0;
-    const int n0 = (unit - group * args.nblk) * 128;
-    int lo = 0, hi = args.rows;
-    if (args.offsets)
-    {
-        const int a = __ldg(args.offsets + group), b = __ldg(args.offsets + group + 1);
-        lo = max(0, min(a, args.rows));
-        hi = max(0, min(b, args.rows));
-        if ((a != lo || b != hi || hi < lo) && threadIdx.x == 0) record_status(args.status, kStatusBadIndex);
-    }
-    // row tiles blockIdx.y, + gridDim.y, ...: the same in every CTA of the cluster
-    const int tiles = hi > lo ? (hi - lo + TN - 1) / TN : 0;
-    if ((int)blockIdx.y >= tiles) return;
+    const int entry = unit / args.nblk;
+    const int n0 = (unit - entry * args.nblk) * 128;
+    const int sharing = args.offsets ? (int)(gridDim.x / S) / args.nblk - args.groups : 0;
+    int other = args.offsets ? entry - args.groups : -1;
+    int group = 0, row0 = 0, live = 0;
+    auto locate = [&]() {
+        int tile = entry, end = args.rows;
+        row0 = 0;
+        if (args.offsets)
+        {
+            group = entry;
+            tile = 0;
+            if (other >= 0)
+            {
+                tile = find_row_tile<TN>(args, other, group);
+                if (tile == 0) return false;
+            }
+            const int a = __ldg(args.offsets + group), b = __ldg(args.offsets + group + 1);
+            row0 = max(0, min(a, args.rows));
+            end = max(0, min(b, args.rows));
+            if ((a != row0 || b != end || end < row0) && threadIdx.x == 0) record_status(args.status, kStatusBadIndex);
+        }
+        row0 += tile * TN;
+        live = min(TN, end - row0);
+        return live > 0;
+    };
+    if (!locate()) return;
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -1076,7 +1133,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 
     int stage = 0;
     uint32_t phase = 0, issued = 0, last_phase = 0;
-    auto load = [&](int kb, int row0) {
+    auto load = [&](int kb) {
         uint8_t* sw = smem + stage * RS::STAGE_BYTES;
         mbar_arrive_expect_tx(&full[stage], RS::STAGE_BYTES);
         tma_load_2d(sw, &tmap_w, &full[stage], kb * BK, group * args.N + n0);
@@ -1089,7 +1146,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
             phase ^= 1;
         }
     };
-    int early = 0; // K blocks of the first row tile already sent for
+    int early = 0; // K blocks already sent for
     if (threadIdx.x == 0)
     {
         for (int s = 0; s < STAGES; s++)
@@ -1108,7 +1165,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         fence_mbarrier_init();
         fence_proxy_async_smem();
         // the ring's first fill does not wait for the set-up below
-        for (; early < STAGES && kb0 + early < kb1; early++) load(kb0 + early, lo + (int)blockIdx.y * TN);
+        for (; early < STAGES && kb0 + early < kb1; early++) load(kb0 + early);
     }
     __syncthreads();
     if (warp == 1) tmem_alloc(tmem_slot, RS::TMEM_COLS);
@@ -1119,10 +1176,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int t = blockIdx.y; t < tiles; t += gridDim.y)
+    for (;;)
     {
-        const int row0 = lo + t * TN;
-        const int live = min(TN, hi - row0);
         if (warp == 0)
         {
             if (lane == 0)
@@ -1130,7 +1185,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
                 for (int kb = kb0 + early; kb < kb1; kb++)
                 {
                     if (!mbar_wait<true>(&empty[stage], phase ^ 1, abort_flag, args.status)) break;
-                    load(kb, row0);
+                    load(kb);
                 }
                 early = 0;
             }
@@ -1213,6 +1268,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
             cluster_sync();
         else
             __syncthreads();
+        if (other < 0) break;
+        other += sharing;
+        if (!locate()) break;
     }
     if (warp == 0 && lane == 0 && *abort_flag)
         for (int s = 0; s < STAGES; s++)
@@ -1312,7 +1370,7 @@ int launch_tiles(Context& ctx, const Operands& o, const BoxMaps& m, LinearArgs a
 }
 
 template <int TN, int S>
-int launch_rows_as(Context& ctx, const Operands& o, const LinearArgs& a, int row_tiles)
+int launch_rows_as(Context& ctx, const Operands& o, const LinearArgs& a, int64_t units)
 {
     using RS = RowsShape<TN>;
     auto kernel = linear_rows_kernel<TN, S>;
@@ -1327,9 +1385,7 @@ int launch_rows_as(Context& ctx, const Operands& o, const LinearArgs& a, int row
         }) != cudaSuccess)
         return S2_ERR_CUDA;
     cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = cluster_config(attr, S, (unsigned)(a.groups * a.nblk * S), kRowsThreads, RS::SMEM_BYTES,
-                                            ctx.stream);
-    cfg.gridDim.y = row_tiles;
+    cudaLaunchConfig_t cfg = cluster_config(attr, S, (unsigned)(units * S), kRowsThreads, RS::SMEM_BYTES, ctx.stream);
     if (cudaLaunchKernelEx(&cfg, kernel, ta, tw, a) != cudaSuccess)
     {
         (void)cudaGetLastError();
@@ -1343,30 +1399,34 @@ template <int TN>
 int launch_rows(Context& ctx, const Operands& o, LinearArgs a)
 {
     a.nblk = (a.N + 127) / 128;
+    // K parts: as many as the resident CTAs leave room for, by the row tiles that
+    // equal groups would have
     const int mean_rows = (a.rows + a.groups - 1) / a.groups;
-    int row_tiles = std::min(65535, (mean_rows + TN - 1) / TN);
-    const int64_t units = (int64_t)a.groups * a.nblk;
-    // K parts: as many as the resident CTAs leave room for; then, for groups of
-    // unknown sizes, CTAs for the row tiles of larger ones (without rows they
-    // return at once; otherwise one CTA takes a group's tiles in turn)
-    const int room = 2 * ctx.num_sms;
+    const int64_t usual = (int64_t)a.groups * ((mean_rows + TN - 1) / TN) * a.nblk;
     int s = 1;
     for (int p : {2, 3, 4, 6, 8})
-        if (p <= a.num_kb && units * row_tiles * p <= room) s = p;
-    if (a.groups > 1 && mean_rows > 8) row_tiles = std::max(row_tiles, 4);
-    if ((int64_t)a.groups * a.nblk * s > 0x7fffffff) return S2_ERR_INVALID;
+        if (p <= a.num_kb && usual * p <= 2 * ctx.num_sms) s = p;
+    // A CTA (or cluster) for each row tile of one group; of several, for each
+    // group's first, and for the others, of which there can be (rows - 1) / TN, as
+    // many as are resident at once.  8,192 rows in 1,024 groups, 512 x 512: all in
+    // one group 137 us (1,886 where a group's CTAs took its tiles in turn, 90 with a
+    // CTA for each tile that there can be), 8 rows in each 113 (105 and 160).
+    const int64_t others = (a.rows - 1) / TN;
+    const int64_t resident = std::max<int64_t>(1, 2 * ctx.num_sms / ((int64_t)a.nblk * s));
+    const int64_t units = (a.groups + (a.offsets ? std::min(others, resident) : others)) * a.nblk;
+    if (units * s > 0x7fffffff) return S2_ERR_INVALID;
     a.chunk_kb = chunk_blocks((a.num_kb + s - 1) / s, a.out_f32);
     const int esz = a.out_f32 ? 4 : 2;
     a.vec_out = reinterpret_cast<uintptr_t>(a.out) % (4 * esz) == 0 && a.out_ld % 4 == 0;
     a.vec_res = reinterpret_cast<uintptr_t>(a.residual) % (4 * esz) == 0 && a.residual_ld % 4 == 0;
     switch (s)
     {
-    case 1: return launch_rows_as<TN, 1>(ctx, o, a, row_tiles);
-    case 2: return launch_rows_as<TN, 2>(ctx, o, a, row_tiles);
-    case 3: return launch_rows_as<TN, 3>(ctx, o, a, row_tiles);
-    case 4: return launch_rows_as<TN, 4>(ctx, o, a, row_tiles);
-    case 6: return launch_rows_as<TN, 6>(ctx, o, a, row_tiles);
-    default: return launch_rows_as<TN, 8>(ctx, o, a, row_tiles);
+    case 1: return launch_rows_as<TN, 1>(ctx, o, a, units);
+    case 2: return launch_rows_as<TN, 2>(ctx, o, a, units);
+    case 3: return launch_rows_as<TN, 3>(ctx, o, a, units);
+    case 4: return launch_rows_as<TN, 4>(ctx, o, a, units);
+    case 6: return launch_rows_as<TN, 6>(ctx, o, a, units);
+    default: return launch_rows_as<TN, 8>(ctx, o, a, units);
     }
 }
 
