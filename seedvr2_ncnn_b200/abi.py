@@ -513,10 +513,11 @@ def _new(ctx, shape, dtype):
     return t
 
 
-def _new_out(ctx, shape, code):
-    import torch
-
-    return _new(ctx, shape, torch.float32 if code == S2_DTYPE_F32 else torch.bfloat16)
+def _new_out(ctx, shape, code, what: str):
+    for dtype, c in _codes.items():
+        if c == code:
+            return _new(ctx, shape, dtype)
+    _refuse(what)  # another number, or a torch type
 
 
 def _operand_stride(t, shape, device: int, what: str) -> int:
@@ -544,7 +545,7 @@ def _linear(ctx, what, a, weight, offsets, bias, act, gate, residual, out_dtype,
         _refuse(what)
     lda, ldw = _operand_stride(a, a_shape, dev, what), _operand_stride(weight, w_shape, dev, what)
     if out is None:
-        out = _new_out(ctx, (rows, N), out_dtype)
+        out = _new_out(ctx, (rows, N), out_dtype, what)
     code = codes.get(out.dtype)
     if code is None or out.shape != (rows, N) or out.get_device() != dev:
         _refuse(what)
@@ -577,7 +578,8 @@ def _linear(ctx, what, a, weight, offsets, bias, act, gate, residual, out_dtype,
 def linear(ctx: Context, a, weight, bias=None, *, act=S2_ACT_NONE, gate=None, residual=None,
            out_dtype=S2_DTYPE_BF16, out=None):
     """residual + gate * act(a @ weight.T + bias): a [M, K] and weight [N, K] bf16 with dense rows of a stride that
-    is a multiple of 8, bias / gate fp32 [N], residual of the output's type (out itself to add in place)."""
+    is a multiple of 8, bias / gate fp32 [N], residual of the output's type (out itself to add in place).  out_dtype:
+    S2_DTYPE_* of the result made here; a given out has its own."""
     return _linear(ctx, "s2_linear", a, weight, None, bias, act, gate, residual, out_dtype, out)
 
 
@@ -592,7 +594,8 @@ def grouped_linear(ctx: Context, a, weight, offsets, bias=None, *, act=S2_ACT_NO
 
 def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=S2_ACT_NONE, out_dtype=None, out=None):
     """act(group norm) of channels-last x [instances, ..., channels] (fp32 or bf16): statistics per instance and
-    channel group over the dimensions between; gamma / beta fp32 [channels].  out: x's shape (x itself in place)."""
+    channel group over the dimensions between; gamma / beta fp32 [channels].  out: x's shape (x itself in place);
+    out_dtype: S2_DTYPE_* of the result made here, x's by default."""
     what = "s2_group_norm"
     dev = ctx.device
     codes = _codes or _dtype_codes()
@@ -607,7 +610,7 @@ def group_norm(ctx: Context, x, groups, gamma=None, beta=None, *, eps=1e-6, act=
     if instances >= 2**31 or channels >= 2**31 or not 0 < groups <= channels:  # a C int drops what it does not hold
         _refuse(what)
     if out is None:
-        out = _new_out(ctx, shape, code if out_dtype is None else out_dtype)
+        out = _new_out(ctx, shape, code if out_dtype is None else out_dtype, what)
     out_code = codes.get(out.dtype)
     if out_code is None or out.shape != shape or out.get_device() != dev:
         _refuse(what)
