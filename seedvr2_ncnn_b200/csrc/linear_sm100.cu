@@ -889,7 +889,8 @@ __global__ void __launch_bounds__(tile_threads(EW, SUM), 1)
 // on the run), applies the epilogue and stores: a warp takes one row's 128
 // features, four a lane.  1 x 2,560 x 2,560 takes 7.0 us (2.0 at the memory's
 // rate: the set-up, one trip to memory and two cluster barriers are the rest), 58 x
-// 10,240 x 2,560 16.0 (8.4), 64 groups of 2,048 x 1,024 at 2 rows 37 = 5.3 TB/s.
+// 10,240 x 2,560 16.0 (8.4), 64 groups of 2,048 x 1,024 at 2 rows each 53 = 5.1
+// TB/s.
 constexpr int kRowsThreads = 192;
 
 template <int TN>
@@ -1478,15 +1479,16 @@ int run_linear(s2_context* ctx, int rows, int groups, const int* offsets, int N,
         const double row_tiles = groups == 1 ? (rows + m - 1) / m : groups * ((double)rows / groups / m + 0.5);
         return row_tiles * ((N + n - 1) / n);
     };
-    // The transposed product, whose K is split over clusters: up to 8 rows a
-    // group (64 groups of 2,048 x 1,024 at 2 rows 37 us, against 44 in tiles;
-    // at 10 rows 61 against 49), up to 64 where the tiles are few (2,560 x
-    // 2,560, 64 rows 9.6 us against 16.7; 16 groups of 2,048 x 2,048 at 19 rows
-    // 24 against 29; 32 of 1,024 x 2,048 at 31 rows, 256 tiles, 35 against 33),
-    // and more rows of one group while half the SMs would have no tile (2,560 x
-    // 2,560: 300 rows 14.2 us against 17.8; 512 rows, 80 tiles, 19.8 against 17.9).
+    // The transposed product, whose K is split over clusters: up to 16 rows a
+    // group (64 groups of 2,048 x 1,024: 2 rows 53 us, against 58 in tiles; 16 rows
+    // 58 and 59, 24 rows 61 and 60; 16 x 51,200 x 2,560 55 and 82), up to 64 where
+    // there are fewer than two tiles a SM (16 groups of 2,048 x 2,048, 256 tiles, at
+    // 64 rows 35 against 37; 32 of 2,560 x 2,560, 480 tiles, at 32 rows 87.3 and
+    // 86.8; 64 x 51,200 x 2,560, 400 tiles, 63 and 59), and more rows of one group
+    // while half the SMs would have no tile (2,560 x 2,560: 300 rows, 60 tiles, 19
+    // us against 21; 512 rows, 80 tiles, 24 and 20).
     const double few = tiles(128, 128);
-    if (mean_rows <= 8 || (mean_rows <= 64 && few < 1.2 * c.num_sms) || (groups == 1 && few < 0.5 * c.num_sms))
+    if (mean_rows <= 16 || (mean_rows <= 64 && few < 2 * c.num_sms) || (groups == 1 && few < 0.5 * c.num_sms))
     {
         // groups somewhat above the mean still fit one row tile
         const int most = groups == 1 ? rows : mean_rows + mean_rows / 2;
