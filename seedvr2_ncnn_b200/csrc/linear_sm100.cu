@@ -1331,7 +1331,12 @@ int launch_tiles(Context& ctx, const Operands& o, const BoxMaps& m, LinearArgs a
     if (r != S2_OK) return r;
     a.nblk = (a.N + BN - 1) / BN;
     a.stages = TL::stages(a.groups);
-    a.group_m = a.K >= 8192 ? 1 : (a.N <= 4096 ? 8 : 16);
+    // M blocks that share a pass over W: sixteen where W is wide (16,384 x 8,192 x
+    // 4,096: 684 us, against 737 for one; 8,000 x 10,240 x 8,192: 907 and 996), one
+    // where a row of units is about a round of them anyway (21,658 x 2,560 x 10,240
+    // with an fp32 residual: 848 us, against 867 for sixteen; x 2,560: 273 and 284;
+    // 16,384 x 4,096 x 4,096: 341 and 345).
+    a.group_m = a.N <= 4096 ? 1 : 16;
     a.chunk_kb = chunk_blocks(a.num_kb, SUM);
     const int64_t units = ((int64_t)a.rows / (CTAS * BM) + a.groups) * a.nblk; // at most
     if (units > 0x7fffffff) return S2_ERR_INVALID;
