@@ -358,6 +358,7 @@ __device__ __forceinline__ void st_cluster_v4(uint32_t addr, float4 v)
 // Rows of its vector column per thread, in registers: two forms of the kernel,
 // since the longer one's code costs a small x 0.3 us.
 constexpr int kHeld = 8, kHeldMost = 12;
+constexpr int kSlabBlocks = 2; // CTAs a SM: the registers must leave room for them (see kSlabCtas)
 
 // Bytes of the reduction: units x pitch.
 size_t red_bytes(int cols, int per_thread)
@@ -371,7 +372,7 @@ size_t slab_smem(int cluster, int groups, int cols, int per_thread)
 }
 
 template <typename TI, typename TO, int V, int K>
-__global__ void __launch_bounds__(kThreads, 1) group_norm_slab_kernel(const GroupNormArgs a)
+__global__ void __launch_bounds__(kThreads, kSlabBlocks) group_norm_slab_kernel(const GroupNormArgs a)
 {
     extern __shared__ __align__(16) uint8_t smem[];
     const int G = a.groups, P = a.parts;
@@ -751,23 +752,24 @@ struct Cut
 
 // How a problem is cut for vectors of V channels (16 or 8 bytes, or 1 where
 // groups, strides or bases do not admit them).
-//   Slab kernel: slices of 64 bytes (more CTAs; 256 x 512 bf16 4.5 us, against
-//   5.0 in slices of 128 bytes and 5.5 with clusters of 8), 8 rows a thread,
-//   clusters as small as hold the rows, and only where all of it is resident at
-//   once: two CTAs a SM for clusters of up to 8 (4,096 x 512 takes 7.7 us so and
-//   11.2 in two kernels), fewer for larger ones, which find less room (6,000 x
-//   512: 8.2 us in clusters of 12, 192 CTAs, 13.1 in clusters of 16; 7,000 x 512
-//   13.6 in clusters of 14, 224 CTAs).  What does not fit so gets up to 12 rows
-//   a thread with the same bound (7,000 x 512 9.0 us, 9,000 x 512 9.7 against
-//   11.7 in two kernels, 4 x 4,400 x 256 8.8 against 12.9; 3 x 3,555 x 320 fp32,
-//   288 CTAs, would take 17.7 against 11.0).
+//   Slab kernel: slices of 64 bytes (more CTAs; 256 x 512 bf16 with SiLU 5.0 us,
+//   against 5.4 in slices of 128 bytes and 5.7 with clusters of 8), 8 rows a
+//   thread, clusters as small as hold the rows, and only where all of it is
+//   resident at once: two CTAs a SM for clusters of up to 8 (8 x 512 x 512 takes
+//   5.8 us so and 8.1 in two kernels, 2,048 x 512 7.2 and 7.7, 4,096 x 512 8.7 and
+//   8.5), fewer for larger ones, which find less room (6,000 x 512: 9.2 us in
+//   clusters of 12, 192 CTAs, 14.2 in clusters of 16; 7,000 x 512 15.1 in clusters
+//   of 14, 224 CTAs).  What does not fit so gets up to 12 rows a thread with the
+//   same bound (7,000 x 512 10.6 us and 9,000 x 512 11.1, against 11.5 and 13.3 in
+//   two kernels; 4 x 4,400 x 256 10.4 and 14.2; 3 x 3,555 x 320 fp32, 288 CTAs,
+//   would take 17.6 against 11.0).
 //   Sums and apply: slices of at most 128 channels, one wave of CTAs (6 x
-//   14,400 x 512 bf16: 45.5 us at 444 parts, 49.9 at 296, 52.8 at 888).
-constexpr int kSlabCtas = 2 * 148, kLongCtas = 192;
+//   14,400 x 512 bf16: 51.5 us at 444 parts, 61 at 296, 56 at 888).
+constexpr int kSlabCtas = kSlabBlocks * 148, kLongCtas = 192;
 constexpr int kPartCtas = kBlocks * 148;
 // Values a CTA at least: with fewer its set-up costs more than it saves (6 x
-// 4,282 x 128 in two kernels 17.7 us at 8,192, 15.0 at 16,384; 1 x 53,217 x 33
-// 12.3 and 14.7).
+// 4,282 x 128 in two kernels 18.0 us at 8,192, 15.7 at 16,384 and 12.5 at 32,768; 1
+// x 53,217 x 33 20.3, 22.0 and 26.1).
 constexpr int kPartMin = 16384;
 
 Cut cut(int64_t instances, int64_t rows, int C, int width, int V)
