@@ -238,17 +238,16 @@ int s2_linear(s2_context* ctx, int M, int N, int K, const void* A, int64_t lda, 
  * video and text weights, experts): rows offsets[g] <= r < offsets[g + 1] use
  * W [groups][N][K] at row g * N of the stride ldw, bias[g] and gate[g].
  * offsets: device int32 [groups + 1], non-decreasing within [0, rows], read
- * when the kernel runs (no host copy); groups may be empty, rows before
- * offsets[0] and from offsets[groups] on are left as they were.  An offset
- * out of order or range leads no access outside the buffers: s2_status then
- * returns -1 and out's rows are unspecified.  groups <= 1024. */
+ * when the kernel runs (no host copy; not to change meanwhile); groups may be
+ * empty, rows before offsets[0] and from offsets[groups] on are left as they
+ * were.  An offset out of order or range leads no access outside the buffers:
+ * s2_status then returns -1 and out's rows are unspecified.  groups <= 1024. */
 int s2_grouped_linear(s2_context* ctx, int rows, int groups, const int* offsets, int N, int K, const void* A,
                       int64_t lda, const void* W, int64_t ldw, const s2_linear_epilogue* epilogue, int out_dtype,
                       void* out, int64_t ldo);
 
-/* Group norm with an activation over channels-last rows (the norm + SiLU in
- * front of every convolution and of the attention of the VAE's blocks, whose
- * graphs are outside the reference tree):
+/* Group norm with an activation over channels-last rows, as s2_vae_mha_forward
+ * and s2_linear take them (s2_conv3d_* work on planes: no direct neighbours):
  *   out[i][r][c] = act((x[i][r][c] - mean) / sqrt(var + eps) * gamma[c] + beta[c])
  * with mean and biased variance of instance i (a frame) over its `rows` rows
  * and the channels / groups consecutive channels of c's group, in fp32.  x:
