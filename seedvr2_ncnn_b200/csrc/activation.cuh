@@ -52,23 +52,23 @@ constexpr double kLog2e = 1.4426950408889634;
 // polynomial of degree 8 with the least relative error over 0 <= a <= 13.3 (4e-8;
 // beyond, e^(-a^2 / 2) is zero), found by reweighted least squares.  Rounding
 // leaves q within (20 + 2 x^2) 2^-24 of itself.  a above 30 is held there (no inf
-// times zero); the first term keeps NaN and +inf.
+// times zero); x / 2 + |x| / 2 keeps NaN and +inf.
 __device__ __forceinline__ float2 gelu_erf(float2 x)
 {
     constexpr float c[9] = {0.729083657f,  0.50933224f,     0.230019256f,   0.0472572222f,  -0.0104795201f,
                             -0.00692950143f, 0.0010774869f, 0.000911422248f, -0.000272206293f};
     const float2 ax = make_float2(fabsf(x.x), fabsf(x.y));
-    const float2 a = make_float2(fminf(ax.x, 30.f), fminf(ax.y, 30.f));
-    const float2 d = __fadd2_rn(a, splat(3.f));
+    const float2 neg = make_float2(fmaxf(-ax.x, -30.f), fmaxf(-ax.y, -30.f)); // -a
+    const float2 d = __ffma2_rn(neg, splat(-1.f), splat(3.f));
     const float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y));
     const float2 s = __ffma2_rn(r, splat(6.f), splat(-1.f));
-    float2 p = splat(c[8]);
+    float2 q = splat(c[8]);
 #pragma unroll
-    for (int i = 7; i >= 0; i--) p = __ffma2_rn(p, s, splat(c[i]));
-    const float2 z2 = __fmul2_rn(__fmul2_rn(a, splat((float)(-0.5 * kLog2e))), a);
-    p = __fmul2_rn(__fmul2_rn(p, r), make_float2(ex2_approx(z2.x), ex2_approx(z2.y)));
-    p = __fmul2_rn(p, a);
-    return make_float2(fmaf(0.5f, x.x + ax.x, -p.x), fmaf(0.5f, x.y + ax.y, -p.y));
+    for (int i = 7; i >= 0; i--) q = __ffma2_rn(q, s, splat(c[i]));
+    const float2 z2 = __fmul2_rn(__fmul2_rn(neg, splat((float)(-0.5 * kLog2e))), neg);
+    q = __fmul2_rn(__fmul2_rn(q, r), make_float2(ex2_approx(z2.x), ex2_approx(z2.y)));
+    const float2 positive = __ffma2_rn(x, splat(0.5f), __fmul2_rn(ax, splat(0.5f))); // max(x, 0), exact
+    return __ffma2_rn(q, neg, positive);
 }
 
 // v = act(v)

@@ -17,7 +17,7 @@ def _values():
     them.  An odd number of them, so that every kernel's last vector is cut."""
     near = torch.cat([torch.linspace(-16, 16, 1025, dtype=torch.float64), torch.linspace(-130, -16, 229, dtype=torch.float64)])
     far = torch.logspace(2, 30, 57, dtype=torch.float64)
-    bad = torch.tensor([math.nan, math.inf, -math.inf, 0.0, -0.0, -1e-30, 1e-30], dtype=torch.float64)
+    bad = torch.tensor([math.nan, math.inf, -math.inf, 0.0, -0.0, -1e-30, 1e-30, 2e38, -2e38], dtype=torch.float64)
     v = torch.cat([near, far, -far, bad]).float()
     order = torch.randperm(v.numel(), generator=torch.Generator().manual_seed(3))
     return v[order].cuda()
@@ -96,7 +96,7 @@ def test_group_norm(s2lib, gpu_ctx, instances, rows, tin, tout, whole, act):
     """A scale of zero leaves the shift, to the last bit, as the argument."""
     beta = _values()
     if whole:
-        beta = torch.cat([beta, beta[:-beta.numel() % 8]])
+        beta = torch.cat([beta, beta[: -beta.numel() % 8]])
     c = beta.numel()
     x = torch.randn(instances, rows, c, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(tin)
     out = torch.empty(instances, rows, c, device="cuda", dtype=tout)
