@@ -7,6 +7,7 @@
 //     split over a thread-block cluster, for few rows a group.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "activation.cuh"
 #include "s2_common.cuh"
@@ -28,9 +29,9 @@ constexpr size_t kSmemLimit = 232448;
 // over K = 10,240).  Where the result is fp32, sums of at most kChunk blocks
 // (8.7e-7, so that an activation's slope keeps it below 1e-6) are therefore
 // added up in fp32 registers (or shared memory), each while the tensor core
-// works on the next one: 21,658 x 2,560 x 10,240 with an fp32 residual takes 886
-// us so (860 at 24 blocks, 920 at 12) and 810 in one sum.  The price is highest
-// where K just passes one sum: x 1,024 236 us against 156.  A bf16 result rounds
+// works on the next one: 21,658 x 2,560 x 10,240 with an fp32 residual takes 854
+// us so (820 at 24 blocks, 867 at 12) and 782 in one sum.  The price is highest
+// where K just passes one sum: x 1,024 203 us against 143.  A bf16 result rounds
 // at 2^-9 and keeps one sum.
 constexpr int kChunk = 14;
 
@@ -445,6 +446,31 @@ __device__ __forceinline__ void finish(const LinearArgs& a, const float* x0, con
     }
 }
 
+// x = the i-th sixteen of N * 16 sums in registers
+template <int N>
+__device__ __forceinline__ void take_piece(const float (&sum)[N / 2][32], int i, float (&x)[16])
+{
+    auto take = [&](auto k) {
+        constexpr int K = decltype(k)::value;
+        if constexpr (K < N)
+        {
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[j] = sum[K / 2][16 * (K % 2) + j];
+        }
+    };
+    switch (i)
+    {
+    case 0: take(std::integral_constant<int, 0>()); break;
+    case 1: take(std::integral_constant<int, 1>()); break;
+    case 2: take(std::integral_constant<int, 2>()); break;
+    case 3: take(std::integral_constant<int, 3>()); break;
+    case 4: take(std::integral_constant<int, 4>()); break;
+    case 5: take(std::integral_constant<int, 5>()); break;
+    case 6: take(std::integral_constant<int, 6>()); break;
+    default: take(std::integral_constant<int, N - 1>()); break;
+    }
+}
+
 // Epilogue of one warp over all of the CTA's units.  Boxes (32 rows x 128
 // bytes of output) run in a fixed sequence; each is combined in one of the
 // warp's R shared-memory boxes and written by one TMA store.  A residual box is
@@ -621,19 +647,24 @@ __device__ __forceinline__ void tile_epilogue(const LinearArgs& a, const CUtenso
                 release_acc();
             }
             if (!ok) break;
-            // unrolled: `sum` stays in registers
-#pragma unroll
-            for (int i = 0; i < COLS / 32; i++)
+            // one body for all pieces, which fits the instruction cache with its
+            // activations (unrolled, 21,658 x 2,560 x 2,560 with an fp32 residual
+            // takes 290 us instead of 265, with erf GELU 431 instead of 297): `sum`
+            // stays in registers, a jump takes out a piece
+#pragma unroll 1
+            for (int i = 0; i < COLS / 16; i++)
             {
-                const int c = c_lo + 32 * i;
-                if (un.n0 + c >= a.N || live_rows <= 0 || !ok) continue;
-                ok = open_box(c);
-                if (!ok) continue;
-                // sixteen columns at a time: no registers for more
-#pragma unroll
-                for (int j = 0; j < 32; j += 16)
-                    finish<16>(a, &sum[i][j], bias, gate, un.n0 + c + j, stg + (q % R) * kBox + lane * 128, sw, j);
-                close_box(c);
+                const int c = c_lo + 16 * i;
+                if (i % 2 == 0)
+                {
+                    if (un.n0 + c >= a.N || live_rows <= 0) break;
+                    ok = open_box(c);
+                    if (!ok) break;
+                }
+                float x[16];
+                take_piece<COLS / 16>(sum, i, x);
+                finish<16>(a, x, bias, gate, un.n0 + c, stg + (q % R) * kBox + lane * 128, sw, 16 * (i % 2));
+                if (i % 2 == 1) close_box(c - 16);
             }
         }
         else
@@ -1515,9 +1546,9 @@ int run_linear(s2_context* ctx, int rows, int groups, const int* offsets, int N,
     // Boxes per epilogue warp: a third one costs an operand stage and pays
     // where the epilogue moves much beside the operands (of 128 x 256 outputs a
     // CTA): from a quarter of their bytes on (288,000 x 256 x 512 with a bf16
-    // residual 111 against 116 us; 21,658 x 2,560 x 1,280: 119 against 116),
-    // for sums from a fifth (21,658 x 2,560 x 2,560 with an fp32 residual 265
-    // against 281 us; x 10,240: 869 against 847).
+    // residual 124 against 134 us; 21,658 x 2,560 x 1,280: 131 against 124),
+    // for sums from a fifth (21,658 x 2,560 x 2,560 with an fp32 residual 293
+    // against 317 us; x 10,240: 896 against 857).
     const double moved = 128.0 * 256 * osz, fed = (double)a.num_kb * 32768;
     if (a.out_f32 && a.num_kb > kChunk)
     {
